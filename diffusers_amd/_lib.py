@@ -69,6 +69,35 @@ class KernelStat(C.Structure):
                 ("bytes", C.c_double)]
 
 
+class OpExec(C.Structure):
+    _fields_ = [("device_id", C.c_int), ("hip_stream", C.c_void_p), ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t)]
+
+
+class LayerNormArgs(C.Structure):
+    _fields_ = [("dtype", C.c_int), ("param_dtype", C.c_int), ("rows", C.c_int64), ("C", C.c_int64), ("ld_x", C.c_int64), ("ld_y", C.c_int64),
+                ("ld_dy", C.c_int64), ("ld_dx", C.c_int64), ("eps", C.c_float), ("x", C.c_void_p), ("gamma", C.c_void_p), ("beta", C.c_void_p),
+                ("y", C.c_void_p), ("mean", C.c_void_p), ("rstd", C.c_void_p), ("dy", C.c_void_p), ("dx", C.c_void_p), ("dgamma", C.c_void_p),
+                ("dbeta", C.c_void_p)]
+
+
+class GatedFfArgs(C.Structure):
+    _fields_ = [("dtype", C.c_int), ("bias_dtype", C.c_int), ("activation", C.c_int), ("M", C.c_int64), ("K", C.c_int64), ("F", C.c_int64),
+                ("ld_x", C.c_int64), ("ld_w", C.c_int64), ("ld_h", C.c_int64), ("ld_dh", C.c_int64), ("ld_dx", C.c_int64), ("ld_dw", C.c_int64),
+                ("x", C.c_void_p), ("weight", C.c_void_p), ("bias", C.c_void_p), ("h", C.c_void_p), ("dh", C.c_void_p), ("dx", C.c_void_p),
+                ("dweight", C.c_void_p), ("dbias", C.c_void_p)]
+
+
+_Strides = C.c_int64 * 3
+
+
+class CrossAttentionArgs(C.Structure):
+    _fields_ = [("dtype", C.c_int), ("B", C.c_int64), ("Sq", C.c_int64), ("Skv", C.c_int64), ("H", C.c_int64), ("Hkv", C.c_int64), ("D", C.c_int64),
+                ("scale", C.c_float), ("q", C.c_void_p), ("k", C.c_void_p), ("v", C.c_void_p), ("o", C.c_void_p), ("lse", C.c_void_p),
+                ("d_o", C.c_void_p), ("dq", C.c_void_p), ("dk", C.c_void_p), ("dv", C.c_void_p), ("q_lens", C.c_void_p), ("kv_lens", C.c_void_p),
+                ("key_mask", C.c_void_p), ("key_mask_stride", C.c_int64), ("q_stride", _Strides), ("k_stride", _Strides), ("v_stride", _Strides),
+                ("o_stride", _Strides), ("do_stride", _Strides), ("dq_stride", _Strides), ("dk_stride", _Strides), ("dv_stride", _Strides)]
+
+
 # every symbol include/sdengine.h declares: name -> (restype, argtypes)
 _vp, _i, _f = C.c_void_p, C.c_int, C.c_float
 SYMBOLS = {
@@ -110,6 +139,15 @@ SYMBOLS = {
     "sde_rng_standard_normal": (_i, [C.c_uint64, C.c_uint64, _vp, C.c_size_t]),
     "sde_rng_chacha_words": (_i, [_vp, _i, _vp, C.c_size_t]),
     "sde_rng_seed_key": (_i, [C.c_uint64, _vp]),
+    "sde_layer_norm_forward": (_i, [C.POINTER(LayerNormArgs), C.POINTER(OpExec)]),
+    "sde_layer_norm_backward": (_i, [C.POINTER(LayerNormArgs), C.POINTER(OpExec)]),
+    "sde_layer_norm_workspace": (_i, [C.POINTER(LayerNormArgs), C.POINTER(C.c_size_t)]),
+    "sde_gated_ff_forward": (_i, [C.POINTER(GatedFfArgs), C.POINTER(OpExec)]),
+    "sde_gated_ff_backward": (_i, [C.POINTER(GatedFfArgs), C.POINTER(OpExec)]),
+    "sde_gated_ff_workspace": (_i, [C.POINTER(GatedFfArgs), _i, C.POINTER(C.c_size_t)]),
+    "sde_cross_attention_forward": (_i, [C.POINTER(CrossAttentionArgs), C.POINTER(OpExec)]),
+    "sde_cross_attention_backward": (_i, [C.POINTER(CrossAttentionArgs), C.POINTER(OpExec)]),
+    "sde_cross_attention_workspace": (_i, [C.POINTER(CrossAttentionArgs), _i, C.POINTER(C.c_size_t)]),
     "sde_profile_enable": (_i, [_vp, _i]),
     "sde_profile_reset": (_i, [_vp]),
     "sde_profile_get": (_i, [_vp, C.POINTER(KernelStat), _i, C.POINTER(_i)]),

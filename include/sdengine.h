@@ -291,6 +291,103 @@ sde_status sde_rng_standard_normal(uint64_t seed, uint64_t skip, float* out, siz
 sde_status sde_rng_chacha_words(const uint8_t key[32], int rounds, uint32_t* out, size_t n_words);
 sde_status sde_rng_seed_key(uint64_t seed, uint8_t key_out[32]);
 
+/* Operators of the transformer block on device tensors, forward and with their gradients ------------------------------------------
+ * The UNet runs layer norm, cross attention and the gated feed-forward inside sde_unet_forward; these calls offer them one by one, for
+ * callers that need gradients (guidance, textual inversion: the gradient with respect to the encoder's states, adapter tuning), prompts of
+ * different lengths in one batch, or single tokens.  No counterpart in the reference (its graphs run inside ORT sessions).  Conventions:
+ *   - every tensor is a DEVICE pointer on `sde_op_exec.device_id`; work is enqueued on `hip_stream` (NULL: the default stream) and the call
+ *     returns without waiting.  Nothing is allocated and no state is kept: calls on different streams, devices or host threads do not meet, and a
+ *     call may be captured into a graph.  The caller's current device is left as it was;
+ *   - `workspace` (256-byte aligned) is scratch for this call: at least what the matching *_workspace says for the same arguments.  It may
+ *     be used again by later work on the same stream, not by work that may run at the same time;
+ *   - dtype: sde_dtype of the tensors.  All sums, statistics and softmax terms are fp32; results are rounded once at the end, operands of a
+ *     product in the backward passes once more.  No atomics: the same call gives the same bits;
+ *   - sizes may be zero; strides and leading dimensions are in ELEMENTS, the last axis has stride 1.  Arguments that are not met are refused with
+ *     SDE_ERR_INVALID_ARGUMENT before anything is enqueued.  Outputs may not overlap inputs unless stated. */
+typedef struct sde_op_exec {
+    int device_id;
+    void* hip_stream;
+    void* workspace;
+    size_t workspace_bytes;
+} sde_op_exec;
+
+/* y = (x - mean) * rstd * gamma + beta over the last axis of x [rows, C].  gamma / beta [C] of param_dtype (= dtype or SDE_F32), each may be
+ * NULL (ones / zeros).  mean / rstd f32 [rows]: outputs of the forward pass (both NULL if not wanted), inputs of the backward pass.  y may be x.
+ * Backward: dx [rows, C], dgamma, dbeta [C] of param_dtype, each may be NULL (not wanted); dx may be dy. */
+typedef struct sde_layer_norm_args {
+    int dtype, param_dtype;
+    int64_t rows, C;
+    int64_t ld_x, ld_y, ld_dy, ld_dx;
+    float eps;
+    const void* x;
+    const void* gamma;
+    const void* beta;
+    void* y;
+    float* mean;
+    float* rstd;
+    const void* dy;
+    void* dx;
+    void* dgamma;
+    void* dbeta;
+} sde_layer_norm_args;
+sde_status sde_layer_norm_forward(const sde_layer_norm_args* a, const sde_op_exec* exec);
+sde_status sde_layer_norm_backward(const sde_layer_norm_args* a, const sde_op_exec* exec);
+/* scratch of the backward pass (the forward pass needs none) */
+sde_status sde_layer_norm_workspace(const sde_layer_norm_args* a, size_t* bytes);
+
+/* h = (x Wv^T + bv) * act(x Wg^T + bg): x [M, K]; weight [2F, K] with the F value rows first, then the F gate rows (the order of the file's
+ * GEGLU projection); bias [2F] of bias_dtype (= dtype or SDE_F32) or NULL; h [M, F].  K and F are multiples of 8 (SDE_F32: 4), all tensors start on
+ * 16 bytes and their leading dimensions are multiples of 16 bytes and less than 8 MB.
+ * Backward: dh [M, F] -> dx [M, K], dweight [2F, K], dbias [2F] of bias_dtype, each may be NULL.  The pre-activations are formed again from x and
+ * weight; the workspace holds the two gradients of the projections ([M, 2F]). */
+typedef enum sde_activation { SDE_ACT_GELU = 0, SDE_ACT_GELU_TANH = 1, SDE_ACT_SILU = 2 } sde_activation;
+typedef struct sde_gated_ff_args {
+    int dtype, bias_dtype, activation;
+    int64_t M, K, F;
+    int64_t ld_x, ld_w, ld_h, ld_dh, ld_dx, ld_dw;
+    const void* x;
+    const void* weight;
+    const void* bias;
+    void* h;
+    const void* dh;
+    void* dx;
+    void* dweight;
+    void* dbias;
+} sde_gated_ff_args;
+sde_status sde_gated_ff_forward(const sde_gated_ff_args* a, const sde_op_exec* exec);
+sde_status sde_gated_ff_backward(const sde_gated_ff_args* a, const sde_op_exec* exec);
+sde_status sde_gated_ff_workspace(const sde_gated_ff_args* a, int backward, size_t* bytes);
+
+/* o = softmax(scale q k^T) v: q, o [B, Sq, H, D]; k, v [B, Skv, Hkv, D]; H a multiple of Hkv (query head h reads key head h / (H / Hkv)).
+ * D <= 256, a multiple of 8 (SDE_F32: 4).  *_stride: strides of B, S and H; all strides multiples of 16 bytes, 64 steps of S and all heads together span less than 2 GB.
+ * q_lens / kv_lens i32 [B] (device) or NULL: queries / keys at or past their sequence's length do not count (a length is taken between 0 and S);
+ * key_mask u8 [B, Skv], rows key_mask_stride apart, or NULL: a key whose byte is 0 does not count.  What does not count is not read.  A query
+ * without a key that counts, and a query that does not count, gives zeros.  scale > 0.
+ * lse f32 [B, Sq, H]: log of the softmax's denominator (-inf where there is no key): output of the forward pass (or NULL), input of the backward pass.
+ * Backward: d_o, o, lse -> dq, dk, dv, each may be NULL; keys and queries that do not count get zeros. */
+typedef struct sde_cross_attention_args {
+    int dtype;
+    int64_t B, Sq, Skv, H, Hkv, D;
+    float scale;
+    const void* q;
+    const void* k;
+    const void* v;
+    void* o;
+    float* lse;
+    const void* d_o;
+    void* dq;
+    void* dk;
+    void* dv;
+    const int32_t* q_lens;
+    const int32_t* kv_lens;
+    const uint8_t* key_mask;
+    int64_t key_mask_stride;
+    int64_t q_stride[3], k_stride[3], v_stride[3], o_stride[3], do_stride[3], dq_stride[3], dk_stride[3], dv_stride[3];
+} sde_cross_attention_args;
+sde_status sde_cross_attention_forward(const sde_cross_attention_args* a, const sde_op_exec* exec);
+sde_status sde_cross_attention_backward(const sde_cross_attention_args* a, const sde_op_exec* exec);
+sde_status sde_cross_attention_workspace(const sde_cross_attention_args* a, int backward, size_t* bytes);
+
 /* Measurement hooks (bench.py) ------------------------------------------------------------- */
 typedef struct sde_kernel_stat {
     char name[48];

@@ -26,6 +26,7 @@ pub const SDE_CB_NONE: c_int = 0; pub const SDE_CB_PROGRESS: c_int = 1; pub cons
 pub const SDE_CB_DECODED: c_int = 3; pub const SDE_CB_APPROXIMATE: c_int = 4;
 pub const SDE_DPM_SOLVER_PP: c_int = 0; pub const SDE_DPM_SOLVER: c_int = 1;
 pub const SDE_DPM_MIDPOINT: c_int = 0; pub const SDE_DPM_HEUN: c_int = 1;
+pub const SDE_ACT_GELU: c_int = 0; pub const SDE_ACT_GELU_TANH: c_int = 1; pub const SDE_ACT_SILU: c_int = 2;
 pub const SDE_NOALLOC_SCRATCH_BYTES: usize = 8 << 20;
 
 #[repr(C)] #[derive(Clone, Copy)]
@@ -71,6 +72,34 @@ pub struct sde_step_output { pub prev_sample: *mut c_float, pub pred_original_sa
 
 #[repr(C)] #[derive(Clone, Copy)]
 pub struct sde_kernel_stat { pub name: [c_char; 48], pub launches: u64, pub total_ms: c_double, pub flops: c_double, pub bytes: c_double }
+
+#[repr(C)] #[derive(Clone, Copy)]
+pub struct sde_op_exec {
+    pub device_id: c_int, pub hip_stream: *mut c_void, pub workspace: *mut c_void, pub workspace_bytes: usize
+}
+
+#[repr(C)] #[derive(Clone, Copy)]
+pub struct sde_layer_norm_args {
+    pub dtype: c_int, pub param_dtype: c_int, pub rows: i64, pub c: i64, pub ld_x: i64, pub ld_y: i64, pub ld_dy: i64, pub ld_dx: i64,
+    pub eps: c_float, pub x: *const c_void, pub gamma: *const c_void, pub beta: *const c_void, pub y: *mut c_void, pub mean: *mut c_float,
+    pub rstd: *mut c_float, pub dy: *const c_void, pub dx: *mut c_void, pub dgamma: *mut c_void, pub dbeta: *mut c_void
+}
+
+#[repr(C)] #[derive(Clone, Copy)]
+pub struct sde_gated_ff_args {
+    pub dtype: c_int, pub bias_dtype: c_int, pub activation: c_int, pub m: i64, pub k: i64, pub f: i64, pub ld_x: i64, pub ld_w: i64,
+    pub ld_h: i64, pub ld_dh: i64, pub ld_dx: i64, pub ld_dw: i64, pub x: *const c_void, pub weight: *const c_void, pub bias: *const c_void,
+    pub h: *mut c_void, pub dh: *const c_void, pub dx: *mut c_void, pub dweight: *mut c_void, pub dbias: *mut c_void
+}
+
+#[repr(C)] #[derive(Clone, Copy)]
+pub struct sde_cross_attention_args {
+    pub dtype: c_int, pub b: i64, pub sq: i64, pub skv: i64, pub h: i64, pub hkv: i64, pub d: i64, pub scale: c_float,
+    pub q: *const c_void, pub k: *const c_void, pub v: *const c_void, pub o: *mut c_void, pub lse: *mut c_float, pub d_o: *const c_void,
+    pub dq: *mut c_void, pub dk: *mut c_void, pub dv: *mut c_void, pub q_lens: *const i32, pub kv_lens: *const i32, pub key_mask: *const u8,
+    pub key_mask_stride: i64, pub q_stride: [i64; 3], pub k_stride: [i64; 3], pub v_stride: [i64; 3], pub o_stride: [i64; 3],
+    pub do_stride: [i64; 3], pub dq_stride: [i64; 3], pub dk_stride: [i64; 3], pub dv_stride: [i64; 3]
+}
 
 extern "C" {
     pub fn sde_last_error() -> *const c_char;
@@ -119,6 +148,16 @@ extern "C" {
     pub fn sde_rng_standard_normal(seed: u64, skip: u64, out: *mut c_float, n: usize) -> c_int;
     pub fn sde_rng_chacha_words(key: *const u8, rounds: c_int, out: *mut u32, n_words: usize) -> c_int;
     pub fn sde_rng_seed_key(seed: u64, key_out: *mut u8) -> c_int;
+    /* operators of the transformer block on device tensors, enqueued on exec.hip_stream */
+    pub fn sde_layer_norm_forward(a: *const sde_layer_norm_args, exec: *const sde_op_exec) -> c_int;
+    pub fn sde_layer_norm_backward(a: *const sde_layer_norm_args, exec: *const sde_op_exec) -> c_int;
+    pub fn sde_layer_norm_workspace(a: *const sde_layer_norm_args, bytes: *mut usize) -> c_int;
+    pub fn sde_gated_ff_forward(a: *const sde_gated_ff_args, exec: *const sde_op_exec) -> c_int;
+    pub fn sde_gated_ff_backward(a: *const sde_gated_ff_args, exec: *const sde_op_exec) -> c_int;
+    pub fn sde_gated_ff_workspace(a: *const sde_gated_ff_args, backward: c_int, bytes: *mut usize) -> c_int;
+    pub fn sde_cross_attention_forward(a: *const sde_cross_attention_args, exec: *const sde_op_exec) -> c_int;
+    pub fn sde_cross_attention_backward(a: *const sde_cross_attention_args, exec: *const sde_op_exec) -> c_int;
+    pub fn sde_cross_attention_workspace(a: *const sde_cross_attention_args, backward: c_int, bytes: *mut usize) -> c_int;
     pub fn sde_profile_enable(e: *mut sde_engine, enable: c_int) -> c_int;
     pub fn sde_profile_reset(e: *mut sde_engine) -> c_int;
     pub fn sde_profile_get(e: *mut sde_engine, out: *mut sde_kernel_stat, capacity: c_int, n_out: *mut c_int) -> c_int;
