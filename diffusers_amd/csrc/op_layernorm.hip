@@ -31,8 +31,33 @@ struct LnDev {
     long long rows, ldx, ldy, lddy, lddx;
     int C, nchunk, log2tpr;
     float eps, inv_c;
-    int pf32;
+    int pf32, pvec;              // parameters are fp32; they can be read 16 bytes at a time
 };
+
+// a lane's VEC parameters from element c on
+template <typename T, int VEC> __device__ __forceinline__ void params_at(const LnDev& p, const void* q, int c, bool in, float other, float (&f)[VEC])
+{
+    if (!q || !in) {
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) f[i] = other;
+        return;
+    }
+    if constexpr (VEC > 1) {
+        if (p.pvec) {
+            if (p.pf32) {
+#pragma unroll
+                for (int i = 0; i < VEC; i += 4) {
+                    const floatx4 v = *(const floatx4*)((const float*)q + c + i);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) f[i + j] = v[j];
+                }
+            } else vec_get<VEC, T>(*(const typename VecOf<T, VEC>::type*)((const T*)q + c), f);
+            return;
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) f[i] = param_at<T>(q, p.pf32, c + i);
+}
 
 template <bool BLOCK> __device__ __forceinline__ void row_sum2(float& a, float& b, int log2tpr, float (*red)[4][2], int buf)
 {
@@ -62,11 +87,8 @@ __global__ __launch_bounds__(kThreads) void ln_fwd_kernel(LnDev p)
     for (int v = 0; v < VPL; ++v) {
         const int c = v * tpr + pos;
         in[v] = c < p.nchunk;
-#pragma unroll
-        for (int i = 0; i < VEC; ++i) {
-            gm[v][i] = in[v] && p.gamma ? param_at<T>(p.gamma, p.pf32, c * VEC + i) : 1.0f;
-            bt[v][i] = in[v] && p.beta ? param_at<T>(p.beta, p.pf32, c * VEC + i) : 0.0f;
-        }
+        params_at<T, VEC>(p, p.gamma, c * VEC, in[v], 1.0f, gm[v]);
+        params_at<T, VEC>(p, p.beta, c * VEC, in[v], 0.0f, bt[v]);
     }
     const long long step = (long long)gridDim.x * rows_pb;
     const long long first = (long long)blockIdx.x * rows_pb;
@@ -131,9 +153,9 @@ __global__ __launch_bounds__(kThreads) void ln_bwd_kernel(LnDev p)
     for (int v = 0; v < VPL; ++v) {
         const int c = v * tpr + pos;
         in[v] = c < p.nchunk;
+        params_at<T, VEC>(p, p.gamma, c * VEC, in[v], 1.0f, gm[v]);
 #pragma unroll
         for (int i = 0; i < VEC; ++i) {
-            gm[v][i] = in[v] && p.gamma ? param_at<T>(p.gamma, p.pf32, c * VEC + i) : 1.0f;
             dg[v][i] = 0.0f;
             db[v][i] = 0.0f;
         }
@@ -292,22 +314,27 @@ template <typename T> __global__ __launch_bounds__(kThreads) void ln_bwd_long_ke
     }
 }
 
-// column sums of part[n][2][C]: a block takes 64 columns, its 4 waves every fourth row, the waves are added in order
-template <typename T> __global__ __launch_bounds__(kThreads) void ln_cols_kernel(const float* part, int n, int C, void* dgamma, void* dbeta, int pf32)
+// column sums of part[n][2][C]: a block takes 64 columns, each of its 16 waves every 16th row, four in flight; the waves are added in order
+template <typename T> __global__ __launch_bounds__(1024) void ln_cols_kernel(const float* part, int n, int C, void* dgamma, void* dbeta, int pf32)
 {
-    __shared__ float s[4][64];
+    __shared__ float s[16][64];
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
     const int c = blockIdx.x * 64 + lane;                  // of 2C
-    float a = 0.0f, b = 0.0f;
-    if (c < 2 * C) {
+    const long long pitch = 2ll * C;
+    float a[4] = {0.f, 0.f, 0.f, 0.f};
+    if (c < pitch) {
         int i = w;
-        for (; i + 4 < n; i += 8) { a += part[(long long)i * 2 * C + c]; b += part[(long long)(i + 4) * 2 * C + c]; }
-        if (i < n) a += part[(long long)i * 2 * C + c];
+        for (; i + 48 < n; i += 64)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) a[j] += part[(i + 16 * j) * pitch + c];
+        for (; i < n; i += 16) a[0] += part[i * pitch + c];
     }
-    s[w][lane] = a + b;
+    s[w][lane] = (a[0] + a[1]) + (a[2] + a[3]);
     __syncthreads();
-    if (w == 0 && c < 2 * C) {
-        const float t = (s[0][lane] + s[1][lane]) + (s[2][lane] + s[3][lane]);
+    if (w == 0 && c < pitch) {
+        float t = s[0][lane];
+#pragma unroll
+        for (int i = 1; i < 16; ++i) t += s[i][lane];
         if (c < C) { if (dgamma) param_put<T>(dgamma, pf32, c, t); }
         else if (dbeta) param_put<T>(dbeta, pf32, c - C, t);
     }
@@ -356,6 +383,7 @@ LnDev ln_dev(const sde_layer_norm_args& a, const LnPlan& p)
     d.rows = a.rows; d.ldx = a.ld_x; d.ldy = a.ld_y; d.lddy = a.ld_dy; d.lddx = a.ld_dx;
     d.C = (int)a.C; d.nchunk = p.nchunk; d.log2tpr = p.log2tpr;
     d.eps = a.eps; d.inv_c = 1.0f / (float)a.C; d.pf32 = a.param_dtype == SDE_F32;
+    d.pvec = (((uintptr_t)a.gamma | (uintptr_t)a.beta) & 15) == 0;
     return d;
 }
 
@@ -403,7 +431,7 @@ void op_layer_norm_forward(const OpCtx& c, const sde_layer_norm_args& a)
     if (a.rows == 0) return;
     const LnPlan p = ln_plan(a, false);
     const int64_t rows_pb = p.vpl && !p.block ? kThreads >> p.log2tpr : 1;
-    const int grid = (int)std::min<int64_t>(cdiv64(a.rows, rows_pb), 2048);
+    const int grid = (int)std::min<int64_t>(cdiv64(a.rows, rows_pb), 1024);
     const LnDev d = ln_dev(a, p);
     op_dispatch(a.dtype, [&](auto t) { ln_run<decltype(t), false>(p, d, grid, c.stream); });
 }
@@ -419,7 +447,7 @@ void op_layer_norm_backward(const OpCtx& c, const sde_layer_norm_args& a)
         typedef decltype(t) T;
         if (grid) ln_run<T, true>(p, d, grid, c.stream);
         if (params) {        // without rows the sums are empty: zeros
-            ln_cols_kernel<T><<<(unsigned)cdiv64(2 * a.C, 64), kThreads, 0, c.stream>>>((const float*)c.ws, grid, (int)a.C, a.dgamma, a.dbeta, d.pf32);
+            ln_cols_kernel<T><<<(unsigned)cdiv64(2 * a.C, 64), 1024, 0, c.stream>>>((const float*)c.ws, grid, (int)a.C, a.dgamma, a.dbeta, d.pf32);
             op_launched("layer norm column sums");
         }
     });

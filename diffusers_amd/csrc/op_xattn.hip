@@ -30,6 +30,7 @@ struct XaDev {
     float* part_o; float* part_ml;              // forward: [splits][B * Hkv][R][D16], [..][2];  dk / dv: part_o = [splits][2][B][Skv][Hkv][D]
     int B, Sq, Skv, H, Hkv, G, D, R;            // R = Sq * G rows of a key head
     int nrb, nkb, splits;
+    int ragged;                                 // lengths are given: workgroups go to the XCDs in turn, so that one long sequence does not fill one XCD
     float scale, scale2;                        // scale2 = scale log2(e)
 };
 
@@ -140,7 +141,7 @@ __global__ __launch_bounds__(NW * 64) void xa_rows_kernel(XaDev p)
     constexpr int ROWS = NW * QT * 16;
     const int tid = threadIdx.x, lane = tid & 63, wid = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int fr = lane & 15, fg = lane >> 4;
-    int id = xcd_chunk(blockIdx.x, gridDim.x);
+    int id = p.ragged ? blockIdx.x : xcd_chunk(blockIdx.x, gridDim.x);
     const int split = id % p.splits; id /= p.splits;
     const int rb = id % p.nrb; id /= p.nrb;
     const int hk = id % p.Hkv, b = id / p.Hkv;
@@ -391,7 +392,7 @@ __global__ __launch_bounds__(NW * 64) void xa_keys_kernel(XaDev p)
     constexpr int KEYS = NW * KTW * 16;
     const int tid = threadIdx.x, lane = tid & 63, wid = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int fr = lane & 15, fg = lane >> 4;
-    int id = xcd_chunk(blockIdx.x, gridDim.x);
+    int id = p.ragged ? blockIdx.x : xcd_chunk(blockIdx.x, gridDim.x);
     const int split = id % p.splits; id /= p.splits;
     const int kbk = id % p.nkb; id /= p.nkb;
     const int hk = id % p.Hkv, b = id / p.Hkv;
@@ -617,6 +618,7 @@ XaDev xa_dev(const sde_cross_attention_args& a)
     d.B = (int)a.B; d.Sq = (int)a.Sq; d.Skv = (int)a.Skv; d.H = (int)a.H; d.Hkv = (int)a.Hkv; d.G = (int)(a.H / a.Hkv); d.D = (int)a.D; d.R = d.Sq * d.G;
     d.scale = a.scale; d.scale2 = a.scale * kLog2e;
     d.splits = 1;
+    d.ragged = a.q_lens || a.kv_lens;
     return d;
 }
 
