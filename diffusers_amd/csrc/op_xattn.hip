@@ -217,8 +217,8 @@ __global__ __launch_bounds__(NW * 64) void xa_rows_kernel(XaDev p)
         int byte = mask_byte(t0 + 1);
         issue(t0, 0, word);
         for (int t = t0; t < t1; ++t) {
-            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-            __syncthreads();
+            wait_loads();
+            meet();
             if (t + 1 < t1) {
                 next = word_of(t + 1, byte);
                 byte = mask_byte(t + 2);
@@ -311,7 +311,7 @@ __global__ __launch_bounds__(NW * 64) void xa_rows_kernel(XaDev p)
             }
             word = next;
             if constexpr (STAGES == 1) {
-                __syncthreads();
+                meet();
                 if (t + 1 < t1) issue(t + 1, 0, word);
             }
         }
@@ -451,8 +451,8 @@ __global__ __launch_bounds__(NW * 64) void xa_keys_kernel(XaDev p)
         for (int t = t0; t < t1; ++t) {
             const int slot = STAGES == 2 ? (t - t0) & 1 : 0;
             settle(slot);
-            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-            __syncthreads();
+            wait_loads();
+            meet();
             if constexpr (STAGES == 2) if (t + 1 < t1) issue(t + 1, slot ^ 1);
             const char* tq = smem + slot * STAGE;
             const char* to = tq + TB;
@@ -488,7 +488,7 @@ __global__ __launch_bounds__(NW * 64) void xa_keys_kernel(XaDev p)
                     for (int j = 0; j < KTW; ++j) { av[d][j] = mma(oc, pp[j].f[s2], av[d][j]); ak[d][j] = mma(qc, ps[j].f[s2], ak[d][j]); }
                 }
             if constexpr (STAGES == 1) {
-                __syncthreads();
+                meet();
                 if (t + 1 < t1) issue(t + 1, 0);
             }
         }

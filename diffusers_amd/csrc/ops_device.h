@@ -53,15 +53,30 @@ __device__ __forceinline__ floatx4 mma(const Frag<float>& a, const Frag<float>& 
 }
 
 // 16 bytes a lane, global memory to LDS, no registers between: lane l of the wave writes lds + 16 l.  Written out so that the waits are the
-// kernels' own (a compiler-visible load into LDS makes every later LDS read wait for all of them).
+// kernels' own (a compiler-visible load into LDS makes every later LDS read wait for all of them).  It stays where it is written.
 __device__ __forceinline__ void dma16(uintx4 rsrc, unsigned voff, unsigned lds)
 {
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(lds), "v"(voff), "s"(rsrc) : "memory");
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(lds), "v"(voff), "s"(rsrc) : "memory", "m0");
 }
-__device__ __forceinline__ uintx4 make_rsrc(const char* p)
+// Waits for this wave's loads (and stores).  The builtin, not text: the compiler has to know that its own loads have arrived too, or it waits again, for the
+// loads into LDS, wherever one of their registers is used next.
+__device__ __forceinline__ void wait_loads()
+{
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_waitcnt(0x0f70);
+    asm volatile("" ::: "memory");
+}
+// every wave of the workgroup is here, with its LDS reads done
+__device__ __forceinline__ void meet()
+{
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+}
+__device__ __forceinline__ uintx4 make_rsrc(const char* p, unsigned bytes = kOob)
 {
     const unsigned long long a = (unsigned long long)p;
-    return uintx4{(unsigned)__builtin_amdgcn_readfirstlane((int)(unsigned)a), (unsigned)__builtin_amdgcn_readfirstlane((int)(unsigned)(a >> 32)), kOob, 0x00020000u};
+    return uintx4{(unsigned)__builtin_amdgcn_readfirstlane((int)(unsigned)a), (unsigned)__builtin_amdgcn_readfirstlane((int)(unsigned)(a >> 32)), (unsigned)__builtin_amdgcn_readfirstlane((int)bytes), 0x00020000u};
 }
 
 // calls f with a value of the element type that `dtype` names
