@@ -1,0 +1,36 @@
+// op_xattn.h — argument block, plan and launchers of cross attention.
+#pragma once
+#include "ops.h"
+
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+constexpr int kTile = 64;                       // keys (rows, for dk / dv) of a tile
+
+struct Strided { const char* p; long long b, s, h; };       // bytes
+struct XaDev {
+    Strided q, k, v, o, dO, dq, dk, dv;
+    const int* q_lens; const int* kv_lens; const unsigned char* mask; long long mask_b;
+    float* lse; float* delta;                   // [B][Sq][H]
+    float* part_o; float* part_ml;              // forward: [splits][B * Hkv][R][D16], [..][2];  dk / dv: part_o = [splits][2][B][Skv][Hkv][D]
+    int B, Sq, Skv, H, Hkv, G, D, R;            // R = Sq * G rows of a key head
+    int nrb, nkb, splits;
+    int rpg;                                    // row blocks of a workgroup (resident kernels)
+    int chunk;                                  // dk / dv: tiles of rows of a part
+    int ragged;                                 // lengths are given: workgroups go to the XCDs in turn, so that one long sequence does not fill one XCD
+    float scale, scale2;                        // scale2 = scale log2(e)
+};
+
+
+// kd: 64-byte steps of the head dimension, nd: 16-column steps of it; nw, qt: waves of a workgroup and 16-row groups of a wave
+struct XaPlan { int kd, nd, nw, qt, nrb, splits, rpg, nkb, key_splits, chunk; };
+// 16-key groups of a wave that owns keys: two where K, V and both gradients of 32 keys fit into its registers
+constexpr int xa_ktw(bool f32, int kd) { return f32 ? (kd >= 4 ? 1 : 2) : (kd >= 3 ? 1 : 2); }
+// waves of a SIMD the registers are shared out for
+constexpr int xa_waves(bool f32, int kd) { return kd >= (f32 ? 8 : 6) ? 1 : 2; }
+// 16-row groups of a wave: two where q, o and the scores of 32 rows fit
+constexpr int xa_qt(int kd) { return kd >= 5 ? 1 : 2; }
+void xa_forward_f16(const OpCtx& c, const XaPlan& p, const XaDev& d);
+void xa_forward_bf16(const OpCtx& c, const XaPlan& p, const XaDev& d);
+void xa_forward_f32(const OpCtx& c, const XaPlan& p, const XaDev& d);
+void xa_backward_f16(const OpCtx& c, const XaPlan& p, const XaDev& d);
+void xa_backward_bf16(const OpCtx& c, const XaPlan& p, const XaDev& d);
+void xa_backward_f32(const OpCtx& c, const XaPlan& p, const XaDev& d);
