@@ -20,14 +20,16 @@ struct XaDev {
 };
 
 
-// kd: 64-byte steps of the head dimension, nd: 16-column steps of it; nw, qt: waves of a workgroup and 16-row groups of a wave
-struct XaPlan { int kd, nd, nw, qt, nrb, splits, rpg, nkb, key_splits, chunk; };
+// kd: 64-byte steps of the head dimension, nd: 16-column steps of it; nw, qt: waves of a workgroup and 16-row groups of a wave; nrb: row blocks, rpg: of a workgroup that keeps all
+// keys (0: they do not fit)
+struct XaRows { int nw, qt, nrb, rpg; };
+struct XaPlan { int kd, nd; XaRows fwd, dq; int splits, nkb, key_splits, chunk; };
 // 16-key groups of a wave that owns keys: two where K, V and both gradients of 32 keys fit into its registers
 constexpr int xa_ktw(bool f32, int kd) { return f32 ? (kd >= 4 ? 1 : 2) : (kd >= 3 ? 1 : 2); }
 // waves of a SIMD the registers are shared out for
 constexpr int xa_waves(bool f32, int kd) { return kd >= (f32 ? 8 : 6) ? 1 : 2; }
-// 16-row groups of a wave: two where q, o and the scores of 32 rows fit
-constexpr int xa_qt(int kd) { return kd >= 5 ? 1 : 2; }
+// 16-row groups of a wave: two where q, o and the scores of 32 rows (dq: do too) fit into 256 registers.  Head size 128, us, one / two groups: forward 140 / 120, dq 159 / 217.
+constexpr int xa_qt(int kd, bool dq) { return kd >= (dq ? 4 : 5) ? 1 : 2; }
 void xa_forward_f16(const OpCtx& c, const XaPlan& p, const XaDev& d);
 void xa_forward_bf16(const OpCtx& c, const XaPlan& p, const XaDev& d);
 void xa_forward_f32(const OpCtx& c, const XaPlan& p, const XaDev& d);

@@ -57,16 +57,24 @@ XaPlan xa_plan(const sde_cross_attention_args& a)
     XaPlan p{};
     xa_shape(a, p);
     const int64_t R = a.Sq * (a.H / a.Hkv), heads = a.B * a.Hkv, ktiles = cdiv64(a.Skv, kTile);
-    p.nw = R <= 16 ? 1 : 4;                       // one wave for single tokens; 16 rows a wave up to 64 rows, more past that
-    p.qt = R <= 64 ? 1 : xa_qt(p.kd);
-    p.nrb = (int)cdiv64(R, p.nw * p.qt * 16);
+    // one wave for single tokens; 16 rows a wave up to 64 rows, more past that
+    auto rows = [&](bool dq) {
+        const int nw = R <= 16 ? 1 : 4, qt = R <= 64 ? 1 : xa_qt(p.kd, dq);
+        return XaRows{nw, qt, (int)cdiv64(R, nw * qt * 16), 0};
+    };
+    p.fwd = rows(false);
+    p.dq = rows(true);
     // the keys are split when the rows leave CUs idle: to about 8 waves for each CU, at least 2 tiles a part
-    const int64_t blocks = heads * p.nrb, want = p.nw == 1 ? 2048 : 512;
+    const int64_t blocks = heads * p.fwd.nrb, want = p.fwd.nw == 1 ? 2048 : 512;
     p.splits = 1;
-    if (blocks < 256 || (p.nw == 1 && blocks < want)) p.splits = (int)std::max<int64_t>(1, std::min<int64_t>({want / blocks, ktiles / 2, 64}));
+    if (blocks < 256 || (p.fwd.nw == 1 && blocks < want)) p.splits = (int)std::max<int64_t>(1, std::min<int64_t>({want / blocks, ktiles / 2, 64}));
     // two tiles of keys or fewer stay in LDS while a workgroup walks blocks of rows over them: as many as leave 4 workgroups to a CU
     const bool two_stages = 2 * 2 * kTile * p.kd * 64 <= 160 * 1024 - 1024;
-    if (R > 64 && ktiles <= 2 && two_stages && p.splits == 1) p.rpg = (int)std::max<int64_t>(1, std::min<int64_t>(blocks / 1024, 16));
+    if (R > 64 && ktiles <= 2 && two_stages) {
+        auto blocks_of = [&](const XaRows& r) { return (int)std::max<int64_t>(1, std::min<int64_t>(heads * r.nrb / 1024, 16)); };
+        p.fwd.rpg = p.splits == 1 ? blocks_of(p.fwd) : 0;
+        p.dq.rpg = blocks_of(p.dq);
+    }
     // dk / dv: parts of equal numbers of row tiles.  Two workgroups to a CU run at once; four times that many parts where lengths are given, so that a long sequence
     // does not keep a few CUs busy alone.
     const int keys = 4 * 16 * xa_ktw(a.dtype == SDE_F32, p.kd);
@@ -115,8 +123,6 @@ void op_cross_attention_forward(const OpCtx& c, const sde_cross_attention_args& 
         return;
     }
     const XaPlan p = xa_plan(a);
-    d.nrb = p.nrb;
-    d.rpg = p.rpg;
     d.splits = p.splits;
     if (p.splits > 1) {
         d.part_o = (float*)c.ws;
@@ -140,8 +146,6 @@ void op_cross_attention_backward(const OpCtx& c, const sde_cross_attention_args&
     }
     const XaPlan p = xa_plan(a);
     d.delta = (float*)c.ws;
-    d.nrb = p.nrb;
-    d.rpg = p.rpg;
     d.nkb = p.nkb;
     d.splits = p.key_splits;
     d.chunk = p.chunk;

@@ -270,15 +270,20 @@ __global__ __launch_bounds__(NW * 64, xa_waves(sizeof(T) == 4, KD)) void xa_rows
                 }
                 float top[QT];
 #pragma unroll
-                for (int q = 0; q < QT; ++q) {
-                    top[q] = -INFINITY;
+                for (int q = 0; q < QT; ++q) top[q] = -INFINITY;
 #pragma unroll
-                    for (int kt = 0; kt < 4; ++kt)
+                for (int kt = 0; kt < 4; ++kt) {
+                    if (!group_on(kt)) continue;
+#pragma unroll
+                    for (int q = 0; q < QT; ++q)
 #pragma unroll
                         for (int r = 0; r < 4; ++r) {
                             if constexpr (!FULL) s[kt][q][r] = key_on(kt, r) ? s[kt][q][r] : -INFINITY;
                             top[q] = fmaxf(top[q], s[kt][q][r]);
                         }
+                }
+#pragma unroll
+                for (int q = 0; q < QT; ++q) {
                     top[q] = fmaxf(top[q], __shfl_xor(top[q], 16));
                     top[q] = fmaxf(top[q], __shfl_xor(top[q], 32)) * p.scale2;
                 }
@@ -298,19 +303,23 @@ __global__ __launch_bounds__(NW * 64, xa_waves(sizeof(T) == 4, KD)) void xa_rows
                         for (int d = 0; d < ND; ++d) acc[d][q] *= alpha;
                     }
                 }
+                float use[QT];
 #pragma unroll
-                for (int q = 0; q < QT; ++q) {
-                    const float use = m[q] == -INFINITY ? 0.0f : m[q];
-                    float sum = 0.0f;
+                for (int q = 0; q < QT; ++q) use[q] = m[q] == -INFINITY ? 0.0f : m[q];
 #pragma unroll
-                    for (int kt = 0; kt < 4; ++kt)
+                for (int kt = 0; kt < 4; ++kt) {
+                    const bool on = group_on(kt);
+#pragma unroll
+                    for (int q = 0; q < QT; ++q) {
+                        float sum = 0.0f;
 #pragma unroll
                         for (int r = 0; r < 4; ++r) {
-                            const float e = __builtin_amdgcn_exp2f(fmaf(s[kt][q][r], p.scale2, -use));
+                            const float e = on ? __builtin_amdgcn_exp2f(fmaf(s[kt][q][r], p.scale2, -use[q])) : 0.0f;
                             sum += e;
                             pf[q].set(kt, r, e);      // rounded to the inputs' type: the operand of the product with v; the sum takes it unrounded
                         }
-                    l[q] += sum;
+                        l[q] += sum;
+                    }
                 }
             } else {
                 auto prob = [&](const floatx4 (&x)[QT], int kt, int q, int r) { return key_on(kt, r) ? __builtin_amdgcn_exp2f(fmaf(x[q][r], p.scale2, -lse2[q])) : 0.0f; };
@@ -338,6 +347,13 @@ __global__ __launch_bounds__(NW * 64, xa_waves(sizeof(T) == 4, KD)) void xa_rows
                 }
 #pragma unroll
                 for (int kt = 0; kt < 4; ++kt) {
+                    if (!group_on(kt)) {
+#pragma unroll
+                        for (int q = 0; q < QT; ++q)
+#pragma unroll
+                            for (int r = 0; r < 4; ++r) pf[q].set(kt, r, 0.0f);
+                        continue;
+                    }
                     floatx4 s[QT], dp[QT];
                     scores(tk, kt, qf, s);
                     scores(tv, kt, of, dp);
@@ -668,15 +684,17 @@ template <typename T, int KD, int ND, int NW, int QT, int MODE, bool RES> void x
     k<<<(unsigned)((long long)d.B * d.Hkv * groups * d.splits), NW * 64, smem, c.stream>>>(d);
     op_launched("cross attention");
 }
-template <typename T, int KD, int ND, int MODE> void xa_rows_by(const OpCtx& c, const XaPlan& p, const XaDev& d)
+template <typename T, int KD, int ND, int MODE> void xa_rows_by(const OpCtx& c, const XaRows& r, XaDev d)
 {
-    constexpr int QT = xa_qt(KD);
-    if (p.nw == 1) { xa_rows<T, KD, ND, 1, 1, MODE, false>(c, d); return; }
+    constexpr int QT = xa_qt(KD, MODE == 2);
+    d.nrb = r.nrb;
+    d.rpg = r.rpg;
+    if (r.nw == 1) { xa_rows<T, KD, ND, 1, 1, MODE, false>(c, d); return; }
     if constexpr (MODE != 1 && stages_of(KD, 0) == 2) {
         if (d.rpg) { xa_rows<T, KD, ND, 4, QT, MODE, true>(c, d); return; }
     }
     if constexpr (QT == 2) {
-        if (p.qt == 2) { xa_rows<T, KD, ND, 4, 2, MODE, false>(c, d); return; }
+        if (r.qt == 2) { xa_rows<T, KD, ND, 4, 2, MODE, false>(c, d); return; }
     }
     xa_rows<T, KD, ND, 4, 1, MODE, false>(c, d);
 }
@@ -695,8 +713,8 @@ template <typename T> void xa_forward_type(const OpCtx& c, const XaPlan& p, cons
 {
     xa_with_shape<T>(p.kd, p.nd, [&](auto kd, auto nd) {
         constexpr int KD = decltype(kd)::value, ND = decltype(nd)::value;
-        if (p.splits == 1) { xa_rows_by<T, KD, ND, 0>(c, p, d); return; }
-        xa_rows_by<T, KD, ND, 1>(c, p, d);
+        if (p.splits == 1) { xa_rows_by<T, KD, ND, 0>(c, p.fwd, d); return; }
+        xa_rows_by<T, KD, ND, 1>(c, p.fwd, d);
         xa_join_kernel<T><<<(unsigned)std::min<long long>(cdiv64((long long)d.B * d.Sq * d.H, 4), 8192), 256, 0, c.stream>>>(d, ND * 16);
         op_launched("cross attention join");
     });
@@ -709,7 +727,7 @@ template <typename T> void xa_backward_type(const OpCtx& c, const XaPlan& p, con
         constexpr int KTW = xa_ktw(sizeof(T) == 4, KD);
         XaDev r = d;
         r.splits = 1;
-        xa_rows_by<T, KD, ND, 2>(c, p, r);
+        xa_rows_by<T, KD, ND, 2>(c, p.dq, r);
         if (!d.dk.p && !d.dv.p) return;
         constexpr int smem = stages_of(KD, 2 * kTile * 4) * (2 * kTile * KD * 64 + 2 * kTile * 4);
         auto k = xa_keys_kernel<T, KD, ND, 4, KTW>;
