@@ -308,17 +308,24 @@ __global__ __launch_bounds__(NW * 64, xa_waves(sizeof(T) == 4, KD)) void xa_rows
                 for (int q = 0; q < QT; ++q) use[q] = m[q] == -INFINITY ? 0.0f : m[q];
 #pragma unroll
                 for (int kt = 0; kt < 4; ++kt) {
-                    const bool on = group_on(kt);
+                    if (group_on(kt)) {
+                        if constexpr (!FULL) asm volatile("");        // a branch, not 16 exponentials thrown away
 #pragma unroll
-                    for (int q = 0; q < QT; ++q) {
-                        float sum = 0.0f;
+                        for (int q = 0; q < QT; ++q) {
+                            float sum = 0.0f;
 #pragma unroll
-                        for (int r = 0; r < 4; ++r) {
-                            const float e = on ? __builtin_amdgcn_exp2f(fmaf(s[kt][q][r], p.scale2, -use[q])) : 0.0f;
-                            sum += e;
-                            pf[q].set(kt, r, e);      // rounded to the inputs' type: the operand of the product with v; the sum takes it unrounded
+                            for (int r = 0; r < 4; ++r) {
+                                const float e = __builtin_amdgcn_exp2f(fmaf(s[kt][q][r], p.scale2, -use[q]));
+                                sum += e;
+                                pf[q].set(kt, r, e);      // rounded to the inputs' type: the operand of the product with v; the sum takes it unrounded
+                            }
+                            l[q] += sum;
                         }
-                        l[q] += sum;
+                    } else {
+#pragma unroll
+                        for (int q = 0; q < QT; ++q)
+#pragma unroll
+                            for (int r = 0; r < 4; ++r) pf[q].set(kt, r, 0.0f);
                     }
                 }
             } else {
