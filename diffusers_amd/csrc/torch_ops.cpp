@@ -6,9 +6,11 @@
 #include <ATen/ATen.h>
 #include <ATen/core/grad_mode.h>
 #include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
+#include <c10/hip/HIPGraphsC10Utils.h>
 #include <pybind11/pybind11.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/python_variable.h>
+#include <torch/csrc/autograd/variable.h>
 #include <torch/csrc/utils/pybind.h>
 
 #include "../../include/sdengine.h"
@@ -95,6 +97,19 @@ struct Exec {                                       // the current stream of the
 // autograd takes no tensor that is not there: one that was left out goes in as x (and gets no gradient), with a mark
 const Tensor& or_x(const Tensor& t, const Tensor& x) { return t.defined() ? t : x; }
 struct Given { bool weight, bias; };
+// A backward pass captured into a graph ends the process if the node that gathers a leaf's gradient still belongs to another stream, as it does while a graph built
+// outside of the capture lives: refused here, where the capture can still be given up in order.
+void leaves_of_this_capture(const Tensor& like, std::initializer_list<const Tensor*> inputs)
+{
+    if (c10::hip::currentStreamCaptureStatusMayInitCtx() == c10::hip::CaptureStatus::None) return;
+    const c10::Stream here = c10::hip::getCurrentHIPStreamMasqueradingAsCUDA(like.device().index()).unwrap();
+    for (const Tensor* t : inputs) {
+        if (!t->defined() || !t->requires_grad() || !t->is_leaf()) continue;
+        const auto node = torch::autograd::impl::try_get_grad_accumulator(*t);
+        if (node && node->stream() && *node->stream() != here)
+            throw std::runtime_error("this call is being captured, and a graph of the same leaves that was built on another stream is alive: let go of it first");
+    }
+}
 // gradients come from kernels autograd does not see: a graph through them would be wrong
 void first_derivative_only()
 {
@@ -185,7 +200,10 @@ Tensor layer_norm(const Tensor& x, const std::optional<Tensor>& weight_, const s
     weight = param(weight, x, c, "weight");
     bias = param(bias, x, c, "bias");
     if (weight.defined() && bias.defined() && weight.scalar_type() != bias.scalar_type()) bad_type("weight and bias have one type");
-    if (at::GradMode::is_enabled() && (wants(x) || wants(weight) || wants(bias))) return LayerNorm::apply(x, or_x(weight, x), or_x(bias, x), Given{weight.defined(), bias.defined()}, eps);
+    if (at::GradMode::is_enabled() && (wants(x) || wants(weight) || wants(bias))) {
+        leaves_of_this_capture(x, {&x, &weight, &bias});
+        return LayerNorm::apply(x, or_x(weight, x), or_x(bias, x), Given{weight.defined(), bias.defined()}, eps);
+    }
     return ln_forward(x, as_rows(x, c, 1), weight, bias, eps, nullptr);
 }
 
@@ -270,7 +288,10 @@ Tensor gated_ff(const Tensor& x, const Tensor& weight, const std::optional<Tenso
     const int64_t k = x.size(-1), f = weight.size(0) / 2;
     if (!k || !f || k % step || f % step) bad_value(text("K and F are positive multiples of ", step, " for ", x.scalar_type()));
     bias = param(bias, x, 2 * f, "bias");
-    if (at::GradMode::is_enabled() && (wants(x) || wants(weight) || wants(bias))) return GatedFf::apply(x, weight, or_x(bias, x), Given{true, bias.defined()}, act);
+    if (at::GradMode::is_enabled() && (wants(x) || wants(weight) || wants(bias))) {
+        leaves_of_this_capture(x, {&x, &weight, &bias});
+        return GatedFf::apply(x, weight, or_x(bias, x), Given{true, bias.defined()}, act);
+    }
     return ff_forward(x, as_rows(x, k, 16), as_rows(weight, k, 16), bias, act);
 }
 
@@ -395,7 +416,10 @@ Tensor cross_attention(const Tensor& q, const Tensor& k, const Tensor& v, const 
             bad_value(text("key_mask is a bool tensor of shape [", b, ", ", skv, "]"));
         if ((skv > 1 && mask.stride(1) != 1) || (b > 1 && mask.stride(0) < skv)) mask = mask.contiguous();
     }
-    if (at::GradMode::is_enabled() && (wants(q) || wants(k) || wants(v))) return CrossAttention::apply(q, k, v, Counts{q_lens, kv_lens, mask}, scale);
+    if (at::GradMode::is_enabled() && (wants(q) || wants(k) || wants(v))) {
+        leaves_of_this_capture(q, {&q, &k, &v});
+        return CrossAttention::apply(q, k, v, Counts{q_lens, kv_lens, mask}, scale);
+    }
     return xa_forward(as_heads(q), as_heads(k), as_heads(v), q_lens, kv_lens, mask, scale, nullptr);
 }
 

@@ -10,7 +10,8 @@ not start on 16 bytes where the operator needs that, is copied first.  The same 
     h = gated_ff(x, weight, bias, activation="gelu")     # GEGLU; "silu": SwiGLU
 
 Calls can be captured into a graph.  A backward pass that is to be captured is taken with ``torch.autograd.grad`` of a forward pass in
-the same capture: ``.backward()`` adds into ``.grad`` through nodes that belong to the stream on which the leaves were first used.
+the same capture: ``.backward()`` adds into ``.grad`` through nodes that belong to the stream on which the leaves were first used.  While a graph of
+the same leaves that was built outside of the capture is alive, a call that would need their gradients is refused (RuntimeError).
 
 A tensor of the wrong shape, device or value raises ValueError, of the wrong type TypeError; what the library itself refuses raises ``_lib.SdeError``.
 """
