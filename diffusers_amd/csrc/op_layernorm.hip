@@ -16,8 +16,12 @@ namespace {
 constexpr int kThreads = 256;
 constexpr int kMaxVplWave = 5, kMaxVplBlock = 8;
 
+// 16 bytes at any element: rows of an odd number of values start anywhere, and the hardware takes a global access at any address
+template <typename T, int VEC> struct Loose { typedef typename VecOf<T, VEC>::type type __attribute__((aligned(alignof(T)))); };
+template <typename T> struct Loose<T, 1> { typedef T type; };
+
 struct LnPlan {
-    int vec;        // elements of an access: 16 bytes' worth, or 1 where C, a stride or a pointer does not allow that
+    int vec;        // elements of an access: 16 bytes' worth, or 1 for rows shorter than that
     int nchunk;     // accesses in a row
     int block;      // 1: a row belongs to the whole block
     int log2tpr;    // lanes of a row (wave variant)
@@ -31,7 +35,7 @@ struct LnDev {
     long long rows, ldx, ldy, lddy, lddx;
     int C, nchunk, log2tpr;
     float eps, inv_c;
-    int pf32, pvec;              // parameters are fp32; they can be read 16 bytes at a time
+    int pf32;                    // parameters are fp32
 };
 
 // a lane's VEC parameters from element c on
@@ -43,20 +47,27 @@ template <typename T, int VEC> __device__ __forceinline__ void params_at(const L
         return;
     }
     if constexpr (VEC > 1) {
-        if (p.pvec) {
-            if (p.pf32) {
+        if (p.pf32) {
 #pragma unroll
-                for (int i = 0; i < VEC; i += 4) {
-                    const floatx4 v = *(const floatx4*)((const float*)q + c + i);
+            for (int i = 0; i < VEC; i += 4) {
+                const floatx4 v = *(const typename Loose<float, 4>::type*)((const float*)q + c + i);
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) f[i + j] = v[j];
-                }
-            } else vec_get<VEC, T>(*(const typename VecOf<T, VEC>::type*)((const T*)q + c), f);
-            return;
-        }
+                for (int j = 0; j < 4; ++j) f[i + j] = v[j];
+            }
+        } else vec_get<VEC, T>(*(const typename Loose<T, VEC>::type*)((const T*)q + c), f);
+        return;
     }
 #pragma unroll
     for (int i = 0; i < VEC; ++i) f[i] = param_at<T>(q, p.pf32, c + i);
+}
+
+// First element of access `chunk` of a row.  The last one of a row that is not whole accesses ends with the row: its first `again` elements belong to the access before and are left
+// out of the sums (their results are written twice, the same both times).
+template <int VEC, bool TAIL> __device__ __forceinline__ int first_of(const LnDev& p, int chunk, int& again)
+{
+    const int c = chunk * VEC, over = c + VEC - p.C;
+    again = TAIL && over > 0 ? over : 0;
+    return c - again;
 }
 
 template <bool BLOCK> __device__ __forceinline__ void row_sum2(float& a, float& b, int log2tpr, float (*red)[4][2], int buf)
@@ -73,22 +84,25 @@ template <bool BLOCK> __device__ __forceinline__ void row_sum2(float& a, float& 
     }
 }
 
-template <typename T, int VEC, int VPL, bool BLOCK>
+// TAIL: the row is not whole accesses
+template <typename T, int VEC, int VPL, bool BLOCK, bool TAIL>
 __global__ __launch_bounds__(kThreads) void ln_fwd_kernel(LnDev p)
 {
-    typedef typename VecOf<T, VEC>::type V;
+    typedef typename Loose<T, VEC>::type V;
     __shared__ float red[2][4][2];
     const int tpr = BLOCK ? kThreads : 1 << p.log2tpr;
     const int pos = threadIdx.x & (tpr - 1), slot = BLOCK ? 0 : threadIdx.x >> p.log2tpr;
     const int rows_pb = BLOCK ? 1 : kThreads >> p.log2tpr;
     float gm[VPL][VEC], bt[VPL][VEC];
     bool in[VPL];
+    int at[VPL], again[VPL];
 #pragma unroll
     for (int v = 0; v < VPL; ++v) {
-        const int c = v * tpr + pos;
-        in[v] = c < p.nchunk;
-        params_at<T, VEC>(p, p.gamma, c * VEC, in[v], 1.0f, gm[v]);
-        params_at<T, VEC>(p, p.beta, c * VEC, in[v], 0.0f, bt[v]);
+        in[v] = v * tpr + pos < p.nchunk;
+        at[v] = first_of<VEC, TAIL>(p, v * tpr + pos, again[v]);
+        if (TAIL && !in[v]) again[v] = VEC;
+        params_at<T, VEC>(p, p.gamma, at[v], in[v], 1.0f, gm[v]);
+        params_at<T, VEC>(p, p.beta, at[v], in[v], 0.0f, bt[v]);
     }
     const long long step = (long long)gridDim.x * rows_pb;
     const long long first = (long long)blockIdx.x * rows_pb;
@@ -97,7 +111,7 @@ __global__ __launch_bounds__(kThreads) void ln_fwd_kernel(LnDev p)
     auto fetch = [&](long long r) {
 #pragma unroll
         for (int v = 0; v < VPL; ++v)
-            if (in[v] && r < p.rows) raw[v] = *(const V*)((const T*)p.x + r * p.ldx + (long long)(v * tpr + pos) * VEC);
+            if (in[v] && r < p.rows) raw[v] = *(const V*)((const T*)p.x + r * p.ldx + at[v]);
             else raw[v] = V{};
     };
     fetch(first + slot);
@@ -111,14 +125,14 @@ __global__ __launch_bounds__(kThreads) void ln_fwd_kernel(LnDev p)
 #pragma unroll
         for (int v = 0; v < VPL; ++v)
 #pragma unroll
-            for (int i = 0; i < VEC; ++i) s += x[v][i];
+            for (int i = 0; i < VEC; ++i) s += !TAIL || i >= again[v] ? x[v][i] : 0.0f;
         row_sum2<BLOCK>(s, q, p.log2tpr, red, 0);
         const float mean = s * p.inv_c;
         s = 0.0f;
 #pragma unroll
         for (int v = 0; v < VPL; ++v)
 #pragma unroll
-            for (int i = 0; i < VEC; ++i) { x[v][i] -= mean; if (in[v]) s = fmaf(x[v][i], x[v][i], s); }
+            for (int i = 0; i < VEC; ++i) { x[v][i] -= mean; s = (TAIL ? i >= again[v] : in[v]) ? fmaf(x[v][i], x[v][i], s) : s; }
         row_sum2<BLOCK>(s, q, p.log2tpr, red, 1);
         const float rstd = 1.0f / sqrtf(s * p.inv_c + p.eps);
         if (r < p.rows) {
@@ -132,16 +146,16 @@ __global__ __launch_bounds__(kThreads) void ln_fwd_kernel(LnDev p)
                 float o[VEC];
 #pragma unroll
                 for (int i = 0; i < VEC; ++i) o[i] = fmaf(x[v][i] * rstd, gm[v][i], bt[v][i]);
-                *(V*)((T*)p.y + r * p.ldy + (long long)(v * tpr + pos) * VEC) = vec_set<VEC, T>(o);
+                *(V*)((T*)p.y + r * p.ldy + at[v]) = vec_set<VEC, T>(o);
             }
         }
     }
 }
 
-template <typename T, int VEC, int VPL, bool BLOCK>
+template <typename T, int VEC, int VPL, bool BLOCK, bool TAIL>
 __global__ __launch_bounds__(kThreads) void ln_bwd_kernel(LnDev p)
 {
-    typedef typename VecOf<T, VEC>::type V;
+    typedef typename Loose<T, VEC>::type V;
     __shared__ float red[2][4][2];
     __shared__ float cols[BLOCK ? 1 : 2 * 64 * VPL * VEC];
     const int tpr = BLOCK ? kThreads : 1 << p.log2tpr;
@@ -149,11 +163,13 @@ __global__ __launch_bounds__(kThreads) void ln_bwd_kernel(LnDev p)
     const int rows_pb = BLOCK ? 1 : kThreads >> p.log2tpr;
     float gm[VPL][VEC], dg[VPL][VEC], db[VPL][VEC];
     bool in[VPL];
+    int at[VPL], again[VPL];
 #pragma unroll
     for (int v = 0; v < VPL; ++v) {
-        const int c = v * tpr + pos;
-        in[v] = c < p.nchunk;
-        params_at<T, VEC>(p, p.gamma, c * VEC, in[v], 1.0f, gm[v]);
+        in[v] = v * tpr + pos < p.nchunk;
+        at[v] = first_of<VEC, TAIL>(p, v * tpr + pos, again[v]);
+        if (TAIL && !in[v]) again[v] = VEC;
+        params_at<T, VEC>(p, p.gamma, at[v], in[v], 1.0f, gm[v]);
 #pragma unroll
         for (int i = 0; i < VEC; ++i) {
             dg[v][i] = 0.0f;
@@ -170,10 +186,9 @@ __global__ __launch_bounds__(kThreads) void ln_bwd_kernel(LnDev p)
         rstd_n = ok ? p.rstd_in[r] : 0.0f;
 #pragma unroll
         for (int v = 0; v < VPL; ++v) {
-            const long long c = (long long)(v * tpr + pos) * VEC;
             if (in[v] && ok) {
-                rx[v] = *(const V*)((const T*)p.x + r * p.ldx + c);
-                ry[v] = *(const V*)((const T*)p.dy + r * p.lddy + c);
+                rx[v] = *(const V*)((const T*)p.x + r * p.ldx + at[v]);
+                ry[v] = *(const V*)((const T*)p.dy + r * p.lddy + at[v]);
             } else { rx[v] = V{}; ry[v] = V{}; }
         }
     };
@@ -195,7 +210,7 @@ __global__ __launch_bounds__(kThreads) void ln_bwd_kernel(LnDev p)
 #pragma unroll
             for (int i = 0; i < VEC; ++i) {
                 xh[v][i] = (xh[v][i] - mean) * rstd;
-                const float g = d[v][i] * gm[v][i];
+                const float g = !TAIL || i >= again[v] ? d[v][i] * gm[v][i] : 0.0f;
                 s1 += g;
                 s2 = fmaf(g, xh[v][i], s2);
                 db[v][i] += d[v][i];
@@ -212,7 +227,7 @@ __global__ __launch_bounds__(kThreads) void ln_bwd_kernel(LnDev p)
                 float o[VEC];
 #pragma unroll
                 for (int i = 0; i < VEC; ++i) o[i] = rstd * (fmaf(d[v][i], gm[v][i], -s1) - xh[v][i] * s2);
-                *(V*)((T*)p.dx + r * p.lddx + (long long)(v * tpr + pos) * VEC) = vec_set<VEC, T>(o);
+                *(V*)((T*)p.dx + r * p.lddx + at[v]) = vec_set<VEC, T>(o);
             }
         }
     }
@@ -224,9 +239,9 @@ __global__ __launch_bounds__(kThreads) void ln_bwd_kernel(LnDev p)
             if (!in[v]) continue;
 #pragma unroll
             for (int i = 0; i < VEC; ++i) {
-                const int c = (v * tpr + pos) * VEC + i;
-                part[c] = dg[v][i];
-                part[p.C + c] = db[v][i];
+                if (TAIL && i < again[v]) continue;
+                part[at[v] + i] = dg[v][i];
+                part[p.C + at[v] + i] = db[v][i];
             }
         }
     } else {
@@ -243,7 +258,8 @@ __global__ __launch_bounds__(kThreads) void ln_bwd_kernel(LnDev p)
                 for (int v = 0; v < VPL; ++v)
 #pragma unroll
                     for (int i = 0; i < VEC; ++i) {
-                        const int c = (v * tpr + pos) * VEC + i;             // < 64 * VPL * VEC: tpr <= 64
+                        if (TAIL && i < again[v]) continue;
+                        const int c = at[v] + i;                             // < C <= 64 * VPL * VEC: tpr <= 64
                         cols[c] = (w ? cols[c] : 0.0f) + dg[v][i];
                         cols[64 * VPL * VEC + c] = (w ? cols[64 * VPL * VEC + c] : 0.0f) + db[v][i];
                     }
@@ -340,18 +356,19 @@ template <typename T> __global__ __launch_bounds__(1024) void ln_cols_kernel(con
     }
 }
 
-LnPlan ln_plan(const sde_layer_norm_args& a, bool backward)
+// accesses of a lane at most
+constexpr int ln_most(int vec, bool block) { return block ? kMaxVplBlock : vec == 8 ? 3 : vec == 4 ? kMaxVplWave : 1; }
+
+LnPlan ln_plan(const sde_layer_norm_args& a)
 {
-    const int e = (int)op_esize(a.dtype), full = 16 / e;
-    auto ok = [&](const void* ptr, int64_t ld) { return !ptr || (((uintptr_t)ptr & 15) == 0 && (a.rows <= 1 || (ld * e) % 16 == 0)); };
-    bool wide = a.C % full == 0 && ok(a.x, a.ld_x);
-    if (backward) wide = wide && ok(a.dy, a.ld_dy) && ok(a.dx, a.ld_dx);
-    else wide = wide && ok(a.y, a.ld_y);
-    LnPlan p{wide ? full : 1, 0, 0, 6, 0};
-    if (a.C / p.vec > (int64_t)kThreads * kMaxVplBlock) return p;
-    p.nchunk = (int)(a.C / p.vec);
-    // few rows: as many lanes as the row has accesses, for the shortest chain of loads; many rows: the split that leaves the fewest lanes idle
-    if (p.nchunk > 64 * kMaxVplWave || (a.rows < 512 && p.nchunk > 64)) {
+    const int full = 16 / (int)op_esize(a.dtype);
+    LnPlan p{a.C >= full ? full : 1, 0, 0, 6, 0};
+    if (cdiv64(a.C, p.vec) > (int64_t)kThreads * kMaxVplBlock) return p;
+    p.nchunk = (int)cdiv64(a.C, p.vec);
+    // few rows: as many lanes as the row has accesses, for the shortest chain of loads; many rows: the split that leaves the fewest lanes idle, with at most 3 accesses of 8 values a
+    // lane (more leave too few registers for other waves: fp16 65536 x 320, forward / backward 24.0 / 54.5 us with 5, 18.5 / 33.9 with 3; fp32's 4 values: 5 are as good as 3)
+    const int most = ln_most(p.vec, false);
+    if (p.nchunk > 64 * most || (a.rows < 512 && p.nchunk > 64)) {
         p.block = 1;
         p.vpl = cdiv(p.nchunk, kThreads);
         if (p.vpl > 5) p.vpl = 8;
@@ -360,7 +377,7 @@ LnPlan ln_plan(const sde_layer_norm_args& a, bool backward)
     int best = 1 << 30;
     for (int l = 3; l <= 6; ++l) {
         const int vpl = cdiv(p.nchunk, 1 << l);
-        if (vpl > kMaxVplWave) continue;
+        if (vpl > most) continue;
         const int cost = a.rows < 512 ? -l : (vpl << l);
         if (cost <= best) { best = cost; p.log2tpr = l; p.vpl = vpl; }
     }
@@ -370,7 +387,7 @@ LnPlan ln_plan(const sde_layer_norm_args& a, bool backward)
 // blocks of the backward pass: two for each CU, fewer when there are few rows
 int ln_bwd_blocks(const sde_layer_norm_args& a)
 {
-    const LnPlan p = ln_plan(a, true);
+    const LnPlan p = ln_plan(a);
     const int64_t rows_pb = p.vpl && !p.block ? kThreads >> p.log2tpr : 1;
     return (int)std::min<int64_t>(cdiv64(a.rows, rows_pb), 512);
 }
@@ -383,7 +400,6 @@ LnDev ln_dev(const sde_layer_norm_args& a, const LnPlan& p)
     d.rows = a.rows; d.ldx = a.ld_x; d.ldy = a.ld_y; d.lddy = a.ld_dy; d.lddx = a.ld_dx;
     d.C = (int)a.C; d.nchunk = p.nchunk; d.log2tpr = p.log2tpr;
     d.eps = a.eps; d.inv_c = 1.0f / (float)a.C; d.pf32 = a.param_dtype == SDE_F32;
-    d.pvec = (((uintptr_t)a.gamma | (uintptr_t)a.beta) & 15) == 0;
     return d;
 }
 
@@ -391,8 +407,15 @@ template <typename T, int VEC, bool BLOCK, bool BWD> void ln_launch(const LnPlan
 {
     auto go = [&](auto vpl) {
         constexpr int N = decltype(vpl)::value;
-        if constexpr (BWD) ln_bwd_kernel<T, VEC, N, BLOCK><<<grid, kThreads, 0, s>>>(d);
-        else ln_fwd_kernel<T, VEC, N, BLOCK><<<grid, kThreads, 0, s>>>(d);
+        if constexpr (N <= ln_most(VEC, BLOCK)) {
+            auto of = [&](auto tail) {
+                if constexpr (BWD) ln_bwd_kernel<T, VEC, N, BLOCK, decltype(tail)::value><<<grid, kThreads, 0, s>>>(d);
+                else ln_fwd_kernel<T, VEC, N, BLOCK, decltype(tail)::value><<<grid, kThreads, 0, s>>>(d);
+            };
+            if constexpr (VEC == 1) of(std::false_type{});
+            else if (d.C % VEC) of(std::true_type{});
+            else of(std::false_type{});
+        }
     };
     switch (p.vpl) {
     case 1: go(std::integral_constant<int, 1>{}); break;
@@ -400,7 +423,7 @@ template <typename T, int VEC, bool BLOCK, bool BWD> void ln_launch(const LnPlan
     case 3: go(std::integral_constant<int, 3>{}); break;
     case 4: go(std::integral_constant<int, 4>{}); break;
     case 5: go(std::integral_constant<int, 5>{}); break;
-    default: if constexpr (BLOCK) go(std::integral_constant<int, 8>{}); break;
+    default: go(std::integral_constant<int, 8>{}); break;
     }
 }
 
@@ -409,10 +432,8 @@ template <typename T, bool BWD> void ln_run(const LnPlan& p, const LnDev& d, int
     if (p.vpl == 0) {
         if constexpr (BWD) ln_bwd_long_kernel<T><<<grid, kThreads, 0, s>>>(d);
         else ln_fwd_long_kernel<T><<<grid, kThreads, 0, s>>>(d);
-    } else if (p.vec == 1) {
-        if (p.block) ln_launch<T, 1, true, BWD>(p, d, grid, s);
-        else ln_launch<T, 1, false, BWD>(p, d, grid, s);
-    } else {
+    } else if (p.vec == 1) ln_launch<T, 1, false, BWD>(p, d, grid, s);          // fewer values than an access
+    else {
         if (p.block) ln_launch<T, kVec<T>, true, BWD>(p, d, grid, s);
         else ln_launch<T, kVec<T>, false, BWD>(p, d, grid, s);
     }
@@ -429,7 +450,7 @@ size_t op_layer_norm_ws_bytes(const sde_layer_norm_args& a)
 void op_layer_norm_forward(const OpCtx& c, const sde_layer_norm_args& a)
 {
     if (a.rows == 0) return;
-    const LnPlan p = ln_plan(a, false);
+    const LnPlan p = ln_plan(a);
     const int64_t rows_pb = p.vpl && !p.block ? kThreads >> p.log2tpr : 1;
     const int grid = (int)std::min<int64_t>(cdiv64(a.rows, rows_pb), 1024);
     const LnDev d = ln_dev(a, p);
@@ -438,7 +459,7 @@ void op_layer_norm_forward(const OpCtx& c, const sde_layer_norm_args& a)
 
 void op_layer_norm_backward(const OpCtx& c, const sde_layer_norm_args& a)
 {
-    const LnPlan p = ln_plan(a, true);
+    const LnPlan p = ln_plan(a);
     LnDev d = ln_dev(a, p);
     const bool params = a.dgamma || a.dbeta;
     const int grid = a.rows ? ln_bwd_blocks(a) : 0;
