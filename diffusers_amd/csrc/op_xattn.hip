@@ -69,8 +69,7 @@ XaPlan xa_plan(const sde_cross_attention_args& a)
     p.splits = 1;
     if (blocks < 256 || (p.fwd.nw == 1 && blocks < want)) p.splits = (int)std::max<int64_t>(1, std::min<int64_t>({want / blocks, ktiles / 2, 64}));
     // two tiles of keys or fewer stay in LDS while a workgroup walks blocks of rows over them: as many as leave 4 workgroups to a CU
-    const bool two_stages = 2 * 2 * kTile * p.kd * 64 <= 160 * 1024 - 1024;
-    if (R > 64 && ktiles <= 2 && two_stages) {
+    if (R > 64 && ktiles <= 2) {
         auto blocks_of = [&](const XaRows& r) { return (int)std::max<int64_t>(1, std::min<int64_t>(heads * r.nrb / 1024, 16)); };
         p.fwd.rpg = p.splits == 1 ? blocks_of(p.fwd) : 0;
         p.dq.rpg = blocks_of(p.dq);
