@@ -290,7 +290,9 @@ __global__ __launch_bounds__(NW * 64, xa_waves(sizeof(T) == 4, KD)) void xa_rows
                     }
                 }
             };
-            Probs<T> pf[QT];
+            // few rows: their time is that of reading the keys, so the probabilities go in as two operands, the rounded value and what rounding took away
+            constexpr bool SPLIT = sizeof(T) == 2 && NW == 1 && MODE < 2;
+            Probs<T> pf[QT], pl[SPLIT ? QT : 1];
             if constexpr (MODE < 2) {
                 floatx4 s[4][QT];
 #pragma unroll
@@ -348,6 +350,7 @@ __global__ __launch_bounds__(NW * 64, xa_waves(sizeof(T) == 4, KD)) void xa_rows
                                 const float e = __builtin_amdgcn_exp2f(fmaf(s[kt][q][r], p.scale2, -use[q]));
                                 sum += e;
                                 pf[q].set(kt, r, e);      // rounded to the inputs' type: the operand of the product with v; the sum takes it unrounded
+                                if constexpr (SPLIT) pl[q].set(kt, r, e - (float)(T)e);
                             }
                             l[q] += sum;
                         }
@@ -355,7 +358,10 @@ __global__ __launch_bounds__(NW * 64, xa_waves(sizeof(T) == 4, KD)) void xa_rows
 #pragma unroll
                         for (int q = 0; q < QT; ++q)
 #pragma unroll
-                            for (int r = 0; r < 4; ++r) pf[q].set(kt, r, 0.0f);
+                            for (int r = 0; r < 4; ++r) {
+                                pf[q].set(kt, r, 0.0f);
+                                if constexpr (SPLIT) pl[q].set(kt, r, 0.0f);
+                            }
                     }
                 }
             } else {
@@ -413,7 +419,10 @@ __global__ __launch_bounds__(NW * 64, xa_waves(sizeof(T) == 4, KD)) void xa_rows
                     for (int d = 0; d < ND; ++d) {
                         const Frag<T> cf = rd.cols(tc, d, s2);
 #pragma unroll
-                        for (int q = 0; q < QT; ++q) acc[d][q] = mma(cf, pf[q].f[s2], acc[d][q]);
+                        for (int q = 0; q < QT; ++q) {
+                            acc[d][q] = mma(cf, pf[q].f[s2], acc[d][q]);
+                            if constexpr (SPLIT) acc[d][q] = mma(cf, pl[q].f[s2], acc[d][q]);
+                        }
                     }
                 }
             }
