@@ -384,12 +384,12 @@ LnPlan ln_plan(const sde_layer_norm_args& a)
     return p;
 }
 
-// blocks of the backward pass: two for each CU, fewer when there are few rows
+// blocks of the backward pass: two for each CU, fewer when there are few rows or when the rows are so long that the partial sums would take more than 256 MB
 int ln_bwd_blocks(const sde_layer_norm_args& a)
 {
     const LnPlan p = ln_plan(a);
     const int64_t rows_pb = p.vpl && !p.block ? kThreads >> p.log2tpr : 1;
-    return (int)std::min<int64_t>(cdiv64(a.rows, rows_pb), 512);
+    return (int)std::min<int64_t>({cdiv64(a.rows, rows_pb), 512, std::max<int64_t>(1, (int64_t(256) << 20) / (8 * a.C))});
 }
 
 LnDev ln_dev(const sde_layer_norm_args& a, const LnPlan& p)

@@ -533,6 +533,8 @@ __global__ __launch_bounds__(NW * 64, xa_waves(sizeof(T) == 4, KD)) void xa_keys
     extern __shared__ __attribute__((aligned(16))) char smem[];
     constexpr int TB = kTile * KD * 64, STAGE = 2 * TB + 2 * kTile * 4, STAGES = stages_of(KD, 2 * kTile * 4);      // Q and dO tiles, then lse and delta of the rows
     constexpr int KEYS = NW * KTW * 16;
+    // fp16 holds probabilities below 2^-14 with fewer bits, and with thousands of keys most are: dv is formed from 2^8 times them
+    constexpr float kUp = std::is_same_v<T, half_t> ? 256.0f : 1.0f;
     const int tid = threadIdx.x, lane = tid & 63, wid = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int fr = lane & 15, fg = lane >> 4;
     int id = p.ragged ? blockIdx.x : xcd_chunk(blockIdx.x, gridDim.x);
@@ -636,7 +638,7 @@ __global__ __launch_bounds__(NW * 64, xa_waves(sizeof(T) == 4, KD)) void xa_keys
 #pragma unroll
                     for (int r = 0; r < 4; ++r) {
                         const float e = __builtin_amdgcn_exp2f(fmaf(s[j][r], p.scale2, -ls[r]));
-                        pp[j].set(rt, r, e);              // a key that does not count has its own column of the results alone: set to zero at the end
+                        pp[j].set(rt, r, kUp == 1.0f ? e : e * kUp);          // a key that does not count has its own column of the results alone: set to zero at the end
                         ps[j].set(rt, r, e * (dp[j][r] - dl[r]));
                     }
             }
@@ -668,7 +670,7 @@ __global__ __launch_bounds__(NW * 64, xa_waves(sizeof(T) == 4, KD)) void xa_keys
         for (int d = 0; d < ND; ++d) {
             const int c = d * 16 + fg * 4;
             if (c >= p.D) continue;
-            const floatx4 none = {0.f, 0.f, 0.f, 0.f}, gk = key_ok[j] ? ak[d][j] * p.scale : none, gv = key_ok[j] ? av[d][j] : none;
+            const floatx4 none = {0.f, 0.f, 0.f, 0.f}, gk = key_ok[j] ? ak[d][j] * p.scale : none, gv = key_ok[j] ? av[d][j] * (1.0f / kUp) : none;
             if (part) { *(floatx4*)(part + c) = gk; *(floatx4*)(part + n + c) = gv; }
             else {
                 T4 wk, wv;

@@ -74,7 +74,7 @@ void check(const sde_cross_attention_args* a)
     need(a->B >= 0 && a->Sq >= 0 && a->Skv >= 0 && a->B < kMaxRows && a->Sq < kMaxRows && a->Skv < kMaxRows - 4096, "cross attention: bad B, Sq or Skv");
     need(a->Hkv > 0 && a->H > 0 && a->H < 65536 && a->H % a->Hkv == 0, "cross attention: H must be a multiple of Hkv");
     need(a->D > 0 && a->D <= 256 && a->D % (16 / (int)op_esize(a->dtype)) == 0, "cross attention: D must be at most 256 and a multiple of 16 bytes");
-    need(a->scale > 0.0f && std::isfinite(a->scale), "cross attention: scale must be positive and finite");
+    need(a->scale > 0.0f && std::isfinite(a->scale * 1.5f), "cross attention: scale must be positive and finite");
     need(a->Sq * (a->H / a->Hkv) < kMaxRows - 4096, "cross attention: too many query rows");
     need(a->B * a->Hkv < (1 << 24), "cross attention: B times Hkv is too large");
     need(!a->key_mask || a->B <= 1 || a->key_mask_stride >= a->Skv, "cross attention: key_mask_stride is less than Skv");

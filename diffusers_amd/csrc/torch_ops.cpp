@@ -408,7 +408,7 @@ Tensor cross_attention(const Tensor& q, const Tensor& k, const Tensor& v, const 
     if (!h || !hk || h % hk || d <= 0 || d > 256 || d % step)
         bad_value(text("H is a multiple of Hkv, and D at most 256 and a multiple of ", step, " for ", q.scalar_type()));
     const double scale = scale_ ? *scale_ : 1.0 / std::sqrt((double)d);
-    if (!(scale > 0.0) || !std::isfinite((float)scale)) bad_value("scale is positive and finite");
+    if (!(scale > 0.0) || !std::isfinite((float)scale * 1.5f)) bad_value("scale is positive and finite");
     q_lens = lengths(q_lens, b, "q_lens");
     kv_lens = lengths(kv_lens, b, "kv_lens");
     if (mask.defined()) {

@@ -153,6 +153,28 @@ def test_cross_attention_of_large_scores():
     check(q * 8, k * 4, v, do, grad=False)
 
 
+@pytest.mark.parametrize("d", [4, 12, 20, 100])
+def test_cross_attention_fp32_in_steps_of_four(d):
+    check(*make(2, 70, 81, 2, 2, d, torch.float32, seed=d))
+
+
+def test_more_sequences_than_lanes():
+    g = torch.Generator(device="cuda").manual_seed(13)
+    q, k, v, do = make(70, 9, 40, 2, 1, 64, torch.bfloat16, seed=13)
+    n = lambda top: torch.randint(0, top + 1, (70,), generator=g, device="cuda", dtype=torch.int32)
+    check(q, k, v, do, n(9), n(40))
+
+
+def test_many_keys_in_fp16():
+    """Probabilities of 2^-13 and far less: below 2^-14 fp16 has fewer bits for them, dv does not suffer from it."""
+    q, k, v, do = make(1, 300, 8000, 1, 1, 64, torch.float16, seed=14)
+    _, _, _, dv = check(q, k, v, do)
+    p = torch.softmax(q[0, :, 0].double() @ k[0, :, 0].double().t() / 8, 1)
+    want = p.t() @ do[0, :, 0].double()
+    # one rounding of the probabilities and one of the result, each at most u = 2^-11, in the 2-norm: sums of 300 roundings of random sign
+    assert ((dv[0, :, 0].double() - want).norm() / want.norm()).item() < 2 * 2.0 ** -11
+
+
 @pytest.mark.parametrize("dtype", ["f16", "f32"])
 def test_cross_attention_of_views(dtype):
     t = T[dtype]
