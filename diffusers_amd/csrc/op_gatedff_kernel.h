@@ -155,6 +155,15 @@ __device__ __forceinline__ float row16_sum(float v)
     return v;
 }
 
+// the lane, formed anew: values that only a tile's ends need do not take registers from the products in between (kept, they were spilled, and reading them back waited for the next
+// tile's loads)
+__device__ __forceinline__ int lane_now()
+{
+    unsigned all;
+    asm volatile("s_mov_b32 %0, -1" : "=s"(all));
+    return __builtin_amdgcn_mbcnt_hi(all, __builtin_amdgcn_mbcnt_lo(all, 0));
+}
+
 template <typename T, bool TRA, bool TRB, int EPI, int ACT, int CFG>
 __global__ __launch_bounds__(TileOf<CFG>::type::threads) void gff_gemm_kernel(GffDev p)
 {
@@ -163,8 +172,8 @@ __global__ __launch_bounds__(TileOf<CFG>::type::threads) void gff_gemm_kernel(Gf
     constexpr int KT = 128 / sizeof(T);         // contraction elements of a K-tile
     constexpr bool PAIR = EPI == GFF_FWD || EPI == GFF_BWD;
     constexpr int HALF = C::NT * 8;             // PAIR: value columns of a wave, then as many gate columns
-    const int tid = threadIdx.x, lane = tid & 63, wid = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int wr = wid / C::WN, wc = wid % C::WN, fr = lane & 15, fg = lane >> 4;
+    const int wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wr = wid / C::WN, wc = wid % C::WN;
+    auto tid_now = [&]() -> int { return PAIR ? wid * 64 + lane_now() : (int)threadIdx.x; };      // the other kernels have registers to keep it in
     const int nk_all = (p.Kc + KT - 1) / KT, units = p.nbm * p.nbn * p.splits;
 
     int tm = 0, tn = 0, ks = 0, kt0 = 0, kt1 = 0;
@@ -185,6 +194,7 @@ __global__ __launch_bounds__(TileOf<CFG>::type::threads) void gff_gemm_kernel(Gf
     constexpr int NA = decltype(sa)::N, NB = decltype(sb)::N;
     auto same = [](int r) { return r; };
     auto aim = [&]() {                          // both operands at the unit's first K-tile
+        const int tid = tid_now();
         const long long m0 = (long long)tm * C::BM, n0 = (long long)tn * (PAIR ? C::BN / 2 : C::BN);
         if constexpr (TRA) sa.init(p.A + m0 * sizeof(T) + (long long)kt0 * KT * p.ldA, p.ldA, (int)min((long long)C::BM, p.rowsA - m0), tid, wid, 0, same);
         else sa.init(p.A + m0 * p.ldA + (long long)kt0 * 128, p.ldA, (int)min((long long)C::BM, p.rowsA - m0), tid, wid, 0, same);
@@ -201,9 +211,9 @@ __global__ __launch_bounds__(TileOf<CFG>::type::threads) void gff_gemm_kernel(Gf
     const unsigned smem0 = (unsigned)(unsigned long long)(__attribute__((address_space(3))) char*)smem, lds0 = smem0 + wid * 1024;
     Reader<T, TRA, C::BM> ra;
     Reader<T, TRB, C::BN> rb;
-    ra.init(wr * C::MT * 16, lane);
-    rb.init(wc * C::NT * 16, lane);
-    auto issue = [&](int j, int left, int slot) {            // the 2 N loads of a K-tile, A's first
+    ra.init(wr * C::MT * 16, lane_now());
+    rb.init(wc * C::NT * 16, lane_now());
+    auto issue = [&](int j, int left, int slot, int tid) {            // the 2 N loads of a K-tile, A's first
         if (j < NA) sa.issue(j, lds0 + slot * C::stage, left, tid);
         else if (j < NA + NB) sb.issue(j - NA, lds0 + slot * C::stage + C::a_bytes, left, tid);
     };
@@ -214,7 +224,7 @@ __global__ __launch_bounds__(TileOf<CFG>::type::threads) void gff_gemm_kernel(Gf
     unit(blockIdx.x);
     aim();
 #pragma unroll
-    for (int j = 0; j < NA + NB; ++j) issue(j, p.Kc - kt0 * KT, 0);
+    for (int j = 0; j < NA + NB; ++j) issue(j, p.Kc - kt0 * KT, 0, tid_now());
     for (int u = blockIdx.x; u < units; u += gridDim.x) {
         unit(u);
         const int tm_ = tm, tn_ = tn, ks_ = ks, k0 = kt0, k1 = kt1;
@@ -238,6 +248,7 @@ __global__ __launch_bounds__(TileOf<CFG>::type::threads) void gff_gemm_kernel(Gf
             }
             const unsigned a = smem0 + slot * C::stage, b = a + C::a_bytes;
             slot ^= 1;
+            const int tid = tid_now();
             // Four phases of a quarter of the products (half the rows, half the K-tile); each reads the fragments of the next one in front of its own products, the first two
             // bring in half of the next K-tile each, so that the matrix unit has work while both are under way.  All loads in the first phase: 5 % slower, a quarter in each
             // phase: up to 6 % (the last ones are waited for too soon).
@@ -259,7 +270,7 @@ __global__ __launch_bounds__(TileOf<CFG>::type::threads) void gff_gemm_kernel(Gf
                     for (int nt = 0; nt < C::NT; ++nt) bf[1][nt] = rb.get(b, nt, 1);
                 }
 #pragma unroll
-                for (int j = 0; j < Q; ++j) issue(ph * Q + j, left, slot);
+                for (int j = 0; j < Q; ++j) issue(ph * Q + j, left, slot, tid);
                 __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
                 for (int mt = 0; mt < MH; ++mt)
@@ -269,6 +280,7 @@ __global__ __launch_bounds__(TileOf<CFG>::type::threads) void gff_gemm_kernel(Gf
             }
         }
 
+        const int lane = tid_now() & 63, fr = lane & 15, fg = lane >> 4;
         const long long m0 = (long long)tm_ * C::BM + wr * C::MT * 16 + fr;
         typedef typename VecOf<T, 4>::type T4;
         if constexpr (PAIR) {
