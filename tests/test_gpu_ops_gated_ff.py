@@ -84,6 +84,24 @@ def test_gated_ff_in_steps_of_four_fp32():
     check(*make(37, 68, 44, torch.float32, seed=1), "gelu")
 
 
+@pytest.mark.parametrize("act", ["gelu", "gelu_tanh", "silu"])
+@pytest.mark.parametrize("dtype", ["f16", "bf16", "f32"])
+def test_gated_ff_small_gates(dtype, act):
+    """A gate of 0 gives exactly 0, and small gates keep their relative precision.  x is 0, so a = 1 and g are the bias, exactly.  act(g) = g c with c
+    near 1 / 2: the tail of the erf form is off by 7.5e-8 < 2 v, the other steps by a few v, so 32 v |g| covers each form, beside the one rounding of h."""
+    t = T[dtype]
+    g = torch.zeros(64, device="cuda", dtype=torch.float64)
+    g[2::2] = 2.0 ** -torch.linspace(4, 14, 31, device="cuda", dtype=torch.float64)
+    g[3::2] = -g[2::2]
+    b = torch.cat([torch.ones_like(g), g]).to(t)
+    x = torch.zeros(40, 64, device="cuda", dtype=t)
+    h = ops.gated_ff(x, make(40, 64, 64, t, seed=5)[1], b, activation=act)
+    g = b[64:].double()
+    want = activation(g, act)[0]
+    assert (h[:, :2] == 0).all()
+    within(h, want.expand(40, 64), (32 * V * g.abs()).expand(40, 64), "h")
+
+
 def test_gated_ff_large_gates():
     """Gates far out on both sides: the activation is the gate itself or nothing, its slope 1 or 0."""
     for act in ("gelu", "gelu_tanh", "silu"):
