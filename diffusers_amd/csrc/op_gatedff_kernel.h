@@ -173,7 +173,9 @@ __global__ __launch_bounds__(TileOf<CFG>::type::threads) void gff_gemm_kernel(Gf
     constexpr bool PAIR = EPI == GFF_FWD || EPI == GFF_BWD;
     constexpr int HALF = C::NT * 8;             // PAIR: value columns of a wave, then as many gate columns
     const int wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wr = wid / C::WN, wc = wid % C::WN;
-    auto tid_now = [&]() -> int { return PAIR ? wid * 64 + lane_now() : (int)threadIdx.x; };      // the other kernels have registers to keep it in
+    // only the largest tile's pair kernels lack the registers to keep it: 163 -> 156 us for fp16 65536 x 320 -> 1280; a small tile would pay for it (2 x 1280 -> 5120: 10.1 -> 10.8)
+    constexpr bool ANEW = PAIR && CFG == 0;
+    auto tid_now = [&]() -> int { return ANEW ? wid * 64 + lane_now() : (int)threadIdx.x; };
     const int nk_all = (p.Kc + KT - 1) / KT, units = p.nbm * p.nbn * p.splits;
 
     int tm = 0, tn = 0, ks = 0, kt0 = 0, kt1 = 0;
@@ -211,8 +213,8 @@ __global__ __launch_bounds__(TileOf<CFG>::type::threads) void gff_gemm_kernel(Gf
     const unsigned smem0 = (unsigned)(unsigned long long)(__attribute__((address_space(3))) char*)smem, lds0 = smem0 + wid * 1024;
     Reader<T, TRA, C::BM> ra;
     Reader<T, TRB, C::BN> rb;
-    ra.init(wr * C::MT * 16, lane_now());
-    rb.init(wc * C::NT * 16, lane_now());
+    ra.init(wr * C::MT * 16, ANEW ? lane_now() : (int)threadIdx.x & 63);
+    rb.init(wc * C::NT * 16, ANEW ? lane_now() : (int)threadIdx.x & 63);
     auto issue = [&](int j, int left, int slot, int tid) {            // the 2 N loads of a K-tile, A's first
         if (j < NA) sa.issue(j, lds0 + slot * C::stage, left, tid);
         else if (j < NA + NB) sb.issue(j - NA, lds0 + slot * C::stage + C::a_bytes, left, tid);
