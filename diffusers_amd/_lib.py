@@ -155,6 +155,7 @@ SYMBOLS = {
     "sde_test_conv": (_i, [_vp, _i, _vp, _i, _i, _i, _i, _vp, _vp, _i, _i, _i, _i, _vp, C.c_size_t]),
     "sde_test_conv_res": (_i, [_vp, _i, _vp, _i, _i, _i, _i, _vp, _vp, _i, _i, _vp, _i, _vp, C.c_size_t]),
     "sde_test_geglu": (_i, [_vp, _i, _vp, _i, _i, _vp, _vp, _i, _i, _vp, C.c_size_t]),
+    "sde_test_gated_ff_plan": (_i, [C.POINTER(GatedFfArgs), _i, C.POINTER(_i), C.POINTER(_i), C.POINTER(C.c_int64)]),
     "sde_test_attention": (_i, [_vp, _i, _vp, _vp, _vp, _i, _i, _i, _i, _i, _vp, C.c_size_t]),
 }
 

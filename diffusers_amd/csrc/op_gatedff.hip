@@ -61,8 +61,8 @@ constexpr int kTileRows[3] = {256, 128, 64}, kResident[3] = {1, 2, 4};       // 
 // 1.6; 64 x 64 0.35 / 0.30, 0.4; fp32, whose matrix instructions take 8 times as long on the same bytes, 7.3 / 7.3, 7; 2.05 / 2.1, 2; 0.66 / 0.575, 0.5.
 // E.g. bf16 x W^T with K = 1280, F = 5120, us for the three tiles: 2 rows 28.5, 13.8, 9.1; 1024 rows 36.5, 46.5, 66.1; 8191 rows 217, 276, 472.
 // A split of the contraction adds a launch and its parts in fp32, written and read at 4 TB/s.
-struct GffPlan { int cfg, splits; };
-GffPlan gff_choose(int64_t rows, int64_t cols, int64_t contraction, int dtype, bool may_split)
+// `pitch`: bytes from row to row of the first operand.  A tile's rows have to lie inside the 2 GB window of its loads: rows past it would come as zeros.
+GffPlan gff_choose(int64_t rows, int64_t cols, int64_t contraction, int dtype, bool may_split, int64_t pitch = 0)
 {
     static const double lat[2][3] = {{1.4, 0.6, 0.35}, {7.3, 2.05, 0.66}}, thr[2][3] = {{1.75, 0.72, 0.30}, {7.3, 2.1, 0.575}}, epi[2][3] = {{7.0, 1.6, 0.4}, {7.0, 2.0, 0.5}};
     const int t = dtype == SDE_F32;
@@ -70,6 +70,7 @@ GffPlan gff_choose(int64_t rows, int64_t cols, int64_t contraction, int dtype, b
     GffPlan best{0, 1};
     double least = 1e300;
     for (int c = 0; c < 3; ++c) {
+        if ((kTileRows[c] - 1) * pitch + 128 > (int64_t)kOob) continue;
         const int64_t tiles = cdiv64(rows, kTileRows[c]) * cdiv64(cols, kTileRows[c]);
         for (int s = 1; s <= (may_split ? 32 : 1); ++s) {
             if (s > 1 && nk / s < 4) break;
@@ -88,7 +89,7 @@ GffWs gff_ws(const sde_gated_ff_args& a)
     GffWs w{};
     const size_t e = op_esize(a.dtype);
     w.first = gff_choose(a.M, 2 * a.F, a.K, a.dtype, false);
-    w.dx = gff_choose(a.M, a.K, 2 * a.F, a.dtype, true);
+    w.dx = gff_choose(a.M, a.K, 2 * a.F, a.dtype, true, 2 * a.F * (int64_t)e);
     w.dw = gff_choose(2 * a.F, a.K, a.M, a.dtype, true);
     w.dag = 0;
     w.cols = op_align((size_t)a.M * 2 * a.F * e);
@@ -124,6 +125,15 @@ template <typename T> void gff_product(const OpCtx& c, GffDev d, int dtype, int 
 }
 
 }  // namespace
+
+GffPlan op_gated_ff_plan(const sde_gated_ff_args& a, int product, int64_t* units)
+{
+    const GffWs w = gff_ws(a);
+    const GffPlan p = product == 0 ? w.first : product == 1 ? w.dx : w.dw;
+    const int64_t rows = product == 2 ? 2 * a.F : a.M, cols = product == 0 ? 2 * a.F : a.K;
+    *units = cdiv64(rows, kTileRows[p.cfg]) * cdiv64(cols, kTileRows[p.cfg]) * p.splits;
+    return p;
+}
 
 size_t op_gated_ff_ws_bytes(const sde_gated_ff_args& a, bool backward)
 {

@@ -186,6 +186,17 @@ sde_status sde_gated_ff_backward(const sde_gated_ff_args* a, const sde_op_exec* 
     });
 }
 
+sde_status sde_test_gated_ff_plan(const sde_gated_ff_args* a, int product, int* tile, int* splits, int64_t* units)
+{
+    return guarded([&] {
+        check(a);
+        need(product >= 0 && product <= 2 && a->M > 0 && tile && splits && units, "gated ff plan: bad product, M or output");
+        const GffPlan p = op_gated_ff_plan(*a, product, units);
+        *tile = p.cfg;
+        *splits = p.splits;
+    });
+}
+
 sde_status sde_cross_attention_workspace(const sde_cross_attention_args* a, int backward, size_t* bytes)
 {
     return guarded([&] {

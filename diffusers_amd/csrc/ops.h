@@ -15,6 +15,8 @@ void op_layer_norm_backward(const OpCtx& c, const sde_layer_norm_args& a);
 size_t op_gated_ff_ws_bytes(const sde_gated_ff_args& a, bool backward);
 void op_gated_ff_forward(const OpCtx& c, const sde_gated_ff_args& a);
 void op_gated_ff_backward(const OpCtx& c, const sde_gated_ff_args& a);
+struct GffPlan { int cfg, splits; };                                               // tile (0 = 256 x 256, 1 = 128 x 128, 2 = 64 x 64) and parts of the contraction
+GffPlan op_gated_ff_plan(const sde_gated_ff_args& a, int product, int64_t* units);  // product: 0 = x W^T, 1 = dx, 2 = dW; units: tiles times parts
 
 size_t op_cross_attention_ws_bytes(const sde_cross_attention_args& a, bool backward);
 void op_cross_attention_forward(const OpCtx& c, const sde_cross_attention_args& a);

@@ -429,6 +429,9 @@ sde_status sde_test_conv_res(sde_engine* e, int naive, const float* x, int NB, i
  * 256x320 kernel, 6 the W-stationary streaming kernel. */
 sde_status sde_test_geglu(sde_engine* e, int naive, const float* x, int M, int K, const float* w, const float* bias, int N,
                           int gelu_tanh, float* out, size_t out_capacity);
+/* How the gated feed-forward would run one of its products on these sizes (a host computation; no device is touched): product 0 = x W^T, 1 = dx, 2 = dweight;
+ * tile 0 = 256 x 256, 1 = 128 x 128, 2 = 64 x 64; splits: parts of the contraction; units: tiles times parts. */
+sde_status sde_test_gated_ff_plan(const sde_gated_ff_args* a, int product, int* tile, int* splits, int64_t* units);
 sde_status sde_test_attention(sde_engine* e, int naive, const float* q, const float* k, const float* v,
                               int NB, int heads, int Sq, int Skv, int d, float* out, size_t out_capacity);
 

@@ -170,6 +170,7 @@ extern "C" {
                              out: *mut c_float, out_capacity: usize) -> c_int;
     pub fn sde_test_geglu(e: *mut sde_engine, naive: c_int, x: *const c_float, m: c_int, k: c_int, w: *const c_float, bias: *const c_float,
                           n: c_int, gelu_tanh: c_int, out: *mut c_float, out_capacity: usize) -> c_int;
+    pub fn sde_test_gated_ff_plan(a: *const sde_gated_ff_args, product: c_int, tile: *mut c_int, splits: *mut c_int, units: *mut i64) -> c_int;
     pub fn sde_test_attention(e: *mut sde_engine, naive: c_int, q: *const c_float, k: *const c_float, v: *const c_float,
                               nb: c_int, heads: c_int, sq: c_int, skv: c_int, d: c_int, out: *mut c_float, out_capacity: usize) -> c_int;
 }
