@@ -110,9 +110,16 @@ void leaves_of_this_capture(const Tensor& like, std::initializer_list<const Tens
             throw std::runtime_error("this call is being captured, and a graph of the same leaves that was built on another stream is alive: let go of it first");
     }
 }
-// gradients come from kernels autograd does not see: a graph through them would be wrong
-void first_derivative_only()
+// forward-mode differentiation: a tangent would be left behind without a word
+void no_tangent(std::initializer_list<const Tensor*> inputs)
 {
+    for (const Tensor* t : inputs)
+        if (t->defined() && t->_fw_grad(0).defined()) throw std::runtime_error("the operators have no forward-mode derivatives: an argument carries a tangent");
+}
+// gradients come from kernels autograd does not see: a graph through them would be wrong
+void first_derivative_only(const Tensor& upstream)
+{
+    no_tangent({&upstream});
     if (at::GradMode::is_enabled()) throw std::runtime_error("the operators have first derivatives only (create_graph is set)");
 }
 
@@ -159,7 +166,7 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
     }
     static variable_list backward(AutogradContext* ctx, const variable_list& grads)
     {
-        first_derivative_only();
+        first_derivative_only(grads[0]);
         const variable_list s = ctx->get_saved_variables();
         const Tensor &x2 = s[0], &weight = s[1], &bias = s[2], &stats = s[3], &dy = grads[0];
         const Tensor d2 = as_rows(dy, x2.size(1), 1);
@@ -196,6 +203,7 @@ Tensor layer_norm(const Tensor& x, const std::optional<Tensor>& weight_, const s
     beside(weight, x, "weight");
     beside(bias, x, "bias");
     if (x.dim() == 0 || x.size(-1) == 0) bad_value("layer_norm needs a last axis that is not empty");
+    no_tangent({&x, &weight, &bias});
     const int64_t c = x.size(-1);
     weight = param(weight, x, c, "weight");
     bias = param(bias, x, c, "bias");
@@ -250,7 +258,7 @@ struct GatedFf : torch::autograd::Function<GatedFf> {
     }
     static variable_list backward(AutogradContext* ctx, const variable_list& grads)
     {
-        first_derivative_only();
+        first_derivative_only(grads[0]);
         const variable_list s = ctx->get_saved_variables();
         const Tensor &x2 = s[0], &w2 = s[1], &bias = s[2], &dh = grads[0];
         sde_gated_ff_args a = ff_args(x2, w2, bias, ctx->saved_data["act"].toInt());
@@ -287,6 +295,7 @@ Tensor gated_ff(const Tensor& x, const Tensor& weight, const std::optional<Tenso
     if (weight.scalar_type() != x.scalar_type()) bad_type(text("weight is ", weight.scalar_type(), ", x is ", x.scalar_type()));
     const int64_t k = x.size(-1), f = weight.size(0) / 2;
     if (!k || !f || k % step || f % step) bad_value(text("K and F are positive multiples of ", step, " for ", x.scalar_type()));
+    no_tangent({&x, &weight, &bias});
     bias = param(bias, x, 2 * f, "bias");
     if (at::GradMode::is_enabled() && (wants(x) || wants(weight) || wants(bias))) {
         leaves_of_this_capture(x, {&x, &weight, &bias});
@@ -360,7 +369,7 @@ struct CrossAttention : torch::autograd::Function<CrossAttention> {
     }
     static variable_list backward(AutogradContext* ctx, const variable_list& grads)
     {
-        first_derivative_only();
+        first_derivative_only(grads[0]);
         const variable_list s = ctx->get_saved_variables();
         const Tensor &q = s[0], &k = s[1], &v = s[2];
         const Tensor d_o = as_heads(grads[0]);
@@ -409,6 +418,7 @@ Tensor cross_attention(const Tensor& q, const Tensor& k, const Tensor& v, const 
         bad_value(text("H is a multiple of Hkv, and D at most 256 and a multiple of ", step, " for ", q.scalar_type()));
     const double scale = scale_ ? *scale_ : 1.0 / std::sqrt((double)d);
     if (!(scale > 0.0) || !std::isfinite((float)scale * 1.5f)) bad_value("scale is positive and finite");
+    no_tangent({&q, &k, &v});
     q_lens = lengths(q_lens, b, "q_lens");
     kv_lens = lengths(kv_lens, b, "kv_lens");
     if (mask.defined()) {

@@ -2,7 +2,7 @@
 
 Each call runs the library's own kernels (``sde_layer_norm_*``, ``sde_gated_ff_*``, ``sde_cross_attention_*`` of include/sdengine.h) on the
 current stream of the tensors' device and returns without waiting.  fp16, bf16 and fp32 tensors on a GPU; there is no CPU form.  The
-functions take part in autograd (first derivatives).  Tensors may be strided views: one whose last axis is not contiguous, or whose rows do
+functions take part in autograd (first derivatives, backward; a tensor that carries a forward-mode tangent is refused).  Tensors may be strided views: one whose last axis is not contiguous, or whose rows do
 not start on 16 bytes where the operator needs that, is copied first.  The same call gives the same bits.
 
     y = layer_norm(x, weight, bias)
