@@ -13,6 +13,9 @@ Calls can be captured into a graph.  A backward pass that is to be captured is t
 the same capture: ``.backward()`` adds into ``.grad`` through nodes that belong to the stream on which the leaves were first used.  While a graph of
 the same leaves that was built outside of the capture is alive, a call that would need their gradients is refused (RuntimeError).
 
+They are registered with torch (``torch.ops.diffusers_amd``), so tracers record a call as one node; a saved trace is loaded in a process in
+which one of them has been called.
+
 A tensor of the wrong shape, device or value raises ValueError, of the wrong type TypeError; what the library itself refuses raises ``_lib.SdeError``.
 """
 from __future__ import annotations
