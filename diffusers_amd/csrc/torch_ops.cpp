@@ -16,11 +16,14 @@
 #include <pybind11/pybind11.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/accumulate_grad.h>
 #include <torch/csrc/autograd/python_variable.h>
 #include <torch/csrc/autograd/variable.h>
 #include <torch/csrc/jit/frontend/tracer.h>
 #include <torch/csrc/utils/pybind.h>
 #include <torch/library.h>
+
+#include <unordered_set>
 
 #include "../../include/sdengine.h"
 
@@ -136,17 +139,48 @@ struct Exec {                                       // the current stream of the
 // autograd takes no tensor that is not there: one that was left out goes in as x (and gets no gradient), with a mark
 const Tensor& or_x(const MaybeTensor& t, const Tensor& x) { return t ? *t : x; }
 struct Given { bool weight, bias; };
-// A backward pass captured into a graph ends the process if the node that gathers a leaf's gradient still belongs to another stream, as it does while a graph built
-// outside of the capture lives: refused here, where the capture can still be given up in order.
+// A backward pass captured into a graph ends the process if a gradient goes to a node that belongs to another stream, as the node that gathers a leaf's gradient does while a graph
+// built outside of the capture lives: refused, where the capture can still be given up in order.
+bool capturing(const Tensor& like)
+{
+    if (!has_memory(like)) return false;
+    const c10::OptionalDeviceGuard on(like.device());          // the status is that of the current device's current stream
+    return c10::hip::currentStreamCaptureStatusMayInitCtx() != c10::hip::CaptureStatus::None;
+}
+c10::Stream stream_of(const Tensor& like) { return c10::hip::getCurrentHIPStreamMasqueradingAsCUDA(like.device().index()).unwrap(); }
+bool elsewhere(torch::autograd::Node* node, c10::Stream here) { return node->stream() && *node->stream() != here; }
+// In the forward pass: the leaves of `inputs`, also those behind views and other steps of this capture.  Steps from outside of it are not looked through: whether
+// their gradients will be asked for is known in the backward pass (below).
 void leaves_of_this_capture(const Tensor& like, std::initializer_list<Tensor> inputs)
 {
-    if (!has_memory(like) || c10::hip::currentStreamCaptureStatusMayInitCtx() == c10::hip::CaptureStatus::None) return;
-    const c10::Stream here = c10::hip::getCurrentHIPStreamMasqueradingAsCUDA(like.device().index()).unwrap();
-    for (const Tensor& t : inputs) {
-        if (!t.defined() || !t.requires_grad() || !t.is_leaf()) continue;
-        const auto node = torch::autograd::impl::try_get_grad_accumulator(t);
-        if (node && node->stream() && *node->stream() != here)
-            throw std::runtime_error("this call is being captured, and a graph of the same leaves that was built on another stream is alive: let go of it first");
+    if (!capturing(like)) return;
+    const c10::Stream here = stream_of(like);
+    std::vector<std::shared_ptr<torch::autograd::Node>> nodes;
+    std::unordered_set<const torch::autograd::Node*> seen;
+    for (const Tensor& t : inputs)
+        if (t.defined() && t.requires_grad()) nodes.push_back(t.is_leaf() ? torch::autograd::impl::try_get_grad_accumulator(t) : t.grad_fn());
+    while (!nodes.empty()) {
+        const auto node = nodes.back();
+        nodes.pop_back();
+        if (!node || !seen.insert(node.get()).second) continue;
+        const bool other = elsewhere(node.get(), here);
+        if (dynamic_cast<torch::autograd::AccumulateGrad*>(node.get())) {
+            if (other) throw std::runtime_error("this call is being captured, and a graph of the same leaves that was built on another stream is alive: let go of it first");
+        } else if (!other) {
+            for (const auto& edge : node->next_edges()) nodes.push_back(edge.function);
+        }
+    }
+}
+// In the backward pass: a gradient for a step that was taken outside of the capture.
+void steps_of_this_capture(const Tensor& upstream)
+{
+    if (!capturing(upstream)) return;
+    const c10::Stream here = stream_of(upstream);
+    const auto node = torch::autograd::get_current_node();
+    for (size_t i = 0; node && i < node->num_outputs(); ++i) {
+        const auto& edge = node->next_edge(i);
+        if (edge.is_valid() && node->task_should_compute_output(i) && elsewhere(edge.function.get(), here))
+            throw std::runtime_error("this backward pass is being captured, and it reaches a step that was taken on another stream: take the whole forward pass inside the capture, or detach()");
     }
 }
 // forward-mode differentiation: a tangent would be left behind without a word
@@ -155,10 +189,11 @@ void no_tangent(std::initializer_list<Tensor> inputs)
     for (const Tensor& t : inputs)
         if (t.defined() && t._fw_grad(0).defined()) throw std::runtime_error("the operators have no forward-mode derivatives: an argument carries a tangent");
 }
-// gradients come from kernels autograd does not see: a graph through them would be wrong
-void first_derivative_only(const Tensor& upstream)
+// In front of every backward pass.  Gradients come from kernels autograd does not see: a graph through them would be wrong
+void check_backward(const Tensor& upstream)
 {
     no_tangent({upstream});
+    steps_of_this_capture(upstream);
     if (at::GradMode::is_enabled()) throw std::runtime_error("the operators have first derivatives only (create_graph is set)");
 }
 // Calls an operator through the dispatcher; `Below`: its CUDA or Meta entry (or a tracer in front of it), not its Autograd entry.
@@ -259,7 +294,7 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
     {
         static const auto back = op<std::tuple<Tensor, Tensor, Tensor>(const Tensor&, const Tensor&, const MaybeTensor&, const MaybeTensor&, const Tensor&, double, Wanted)>(
             "diffusers_amd::_layer_norm_backward");
-        first_derivative_only(grads[0]);
+        check_backward(grads[0]);
         const variable_list s = ctx->get_saved_variables();
         Below below;
         auto [dx, dw, db] = back.call(grads[0], s[0], maybe(s[1]), maybe(s[2]), s[3], ctx->saved_data["eps"].toDouble(),
@@ -367,7 +402,7 @@ struct GatedFf : torch::autograd::Function<GatedFf> {
     static variable_list backward(AutogradContext* ctx, const variable_list& grads)
     {
         static const auto back = op<std::tuple<Tensor, Tensor, Tensor>(const Tensor&, const Tensor&, const Tensor&, const MaybeTensor&, int64_t, Wanted)>("diffusers_amd::_gated_ff_backward");
-        first_derivative_only(grads[0]);
+        check_backward(grads[0]);
         const variable_list s = ctx->get_saved_variables();
         Below below;
         auto [dx, dw, db] = back.call(grads[0], s[0], s[1], maybe(s[2]), ctx->saved_data["act"].toInt(),
@@ -532,7 +567,7 @@ struct CrossAttention : torch::autograd::Function<CrossAttention> {
     {
         static const auto back = op<std::tuple<Tensor, Tensor, Tensor>(const Tensor&, const Tensor&, const Tensor&, const Tensor&, const Tensor&, const Tensor&, const MaybeTensor&,
                                                                        const MaybeTensor&, const MaybeTensor&, double, Wanted)>("diffusers_amd::_cross_attention_backward");
-        first_derivative_only(grads[0]);
+        check_backward(grads[0]);
         const variable_list s = ctx->get_saved_variables();
         Below below;
         auto [dq, dk, dv] = back.call(grads[0], s[0], s[1], s[2], s[3], s[4], maybe(s[5]), maybe(s[6]), maybe(s[7]), ctx->saved_data["scale"].toDouble(),

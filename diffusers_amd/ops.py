@@ -11,7 +11,8 @@ not start on 16 bytes where the operator needs that, is copied first.  The same 
 
 Calls can be captured into a graph.  A backward pass that is to be captured is taken with ``torch.autograd.grad`` of a forward pass in
 the same capture: ``.backward()`` adds into ``.grad`` through nodes that belong to the stream on which the leaves were first used.  While a graph of
-the same leaves that was built outside of the capture is alive, a call that would need their gradients is refused (RuntimeError).
+the same leaves that was built outside of the capture is alive, a call that would need their gradients, directly or through views and other steps of the capture, is
+refused (RuntimeError); so is a captured backward pass that reaches a step taken outside of the capture.
 
 They are registered with torch (``torch.ops.diffusers_amd``), so tracers record a call as one node; a saved trace is loaded in a process in
 which one of them has been called.
