@@ -142,6 +142,23 @@ template <typename T> struct Probs {
     }
 };
 
+// Score gradients ds = p (dp - delta) as fp16 operands.  p is about 1 / Skv and the upstream gradient any size, so ds itself lies where fp16 has few bits or none (2^-24 and less: with 8000 keys
+// and do of 1e-3 the products with it were 1 % off) or past its largest value.  They go in as 2^n ds, each column of the product (a row for dq, a key for dk) with an n of its own: it starts
+// high and comes down, with the sums so far, when a value passes 2^15, to put that value at 2^8 .. 2^9.  Powers of two: exact.  bf16 and fp32 have the range.
+// dk / dv: starts at 2^80, the first tile brings it down.  Backward pass of fp16, us before / with: 8 x 2047 x 16 heads of 128 (4 shared) on 1500 keys 908 / 890, 16 x 4096 x 8 of 40 on 77
+// 96 / 100, 2 x 4096 x 8 of 40 on 4096 257 / 259.
+template <typename T> constexpr bool kScaled = std::is_same_v<T, half_t>;
+constexpr float kUpStart = 1.2089258196146292e24f, kUpLimit = 32768.0f;      // 2^80: times the largest |dp - delta| (256 products of 65504^2) it is still finite
+__device__ __forceinline__ unsigned exponent(float m) { return __builtin_bit_cast(unsigned, m) >> 23; }          // of m >= 0: 127 and up from 1, 255 for infinity
+__device__ __forceinline__ float to_2_8(unsigned e) { return __builtin_bit_cast(float, (127 + 8 + 127 - e) << 23); }      // brings a value of this exponent to 2^8 .. 2^9
+// what a column is multiplied with so that its largest magnitude (this lane's is `m`; a column is lanes l, l + 16, + 32, + 48) fits
+__device__ __forceinline__ float fit(float m)
+{
+    m = fmaxf(m, __shfl_xor(m, 16));
+    m = fmaxf(m, __shfl_xor(m, 32));
+    return m > kUpLimit ? to_2_8(exponent(m)) : 1.0f;
+}
+
 // The sequence with the rank-th most keys (none for sequences without queries).  A workgroup's time goes with its sequence's keys; with the longest first, none starts late: bf16, 8
 // ragged sequences of up to 2047 x 16 rows and 1500 keys, forward 107 us in the given order, 100 in this one, 93 with a key head's workgroups on one XCD (below).
 __device__ __forceinline__ int by_length(const XaDev& p, int rank, int lane)
@@ -235,7 +252,7 @@ __global__ __launch_bounds__(NW * 64, xa_waves(sizeof(T) == 4, KD)) void xa_rows
         int rr[QT], rs[QT], rh[QT];
         bool row_in[QT], row_ok[QT];
         Frag<T> qf[QT][KD], of[MODE == 2 ? QT : 1][KD];
-        float lse2[QT], dlt[QT];
+        float lse2[QT], dlt[QT], up[QT];          // up: kScaled
 #pragma unroll
         for (int t = 0; t < QT; ++t) {
             rr[t] = row0 + t * 16 + fr;
@@ -250,10 +267,20 @@ __global__ __launch_bounds__(NW * 64, xa_waves(sizeof(T) == 4, KD)) void xa_rows
                 Frag<T> out[KD];
                 load_rows<T, KD>(of[t], p.dO.p + b * p.dO.b + rs[t] * p.dO.s + rh[t] * p.dO.h, row_ok[t], p.D, lane);
                 load_rows<T, KD>(out, p.o.p + b * p.o.b + rs[t] * p.o.s + rh[t] * p.o.h, row_ok[t], p.D, lane);
+                float size = 0.0f;
 #pragma unroll
                 for (int kk = 0; kk < KD; ++kk)
 #pragma unroll
-                    for (int e = 0; e < kVec<T>; ++e) dlt[t] = fmaf((float)of[t][kk].v[e], (float)out[kk].v[e], dlt[t]);
+                    for (int e = 0; e < kVec<T>; ++e) {
+                        dlt[t] = fmaf((float)of[t][kk].v[e], (float)out[kk].v[e], dlt[t]);
+                        if constexpr (kScaled<T>) size += fabsf((float)of[t][kk].v[e]);
+                    }
+                if constexpr (kScaled<T>) {
+                    // |ds| is at most sum |do| times twice the largest |v|: right at once unless values pass 2^6, when a tile is formed twice
+                    size += __shfl_xor(size, 16);
+                    size += __shfl_xor(size, 32);
+                    up[t] = to_2_8(max(exponent(size), 127u - 24u));
+                }
                 dlt[t] += __shfl_xor(dlt[t], 16);
                 dlt[t] += __shfl_xor(dlt[t], 32);
                 const float l = row_ok[t] ? p.lse[((long long)b * p.Sq + rs[t]) * p.H + rh[t]] : INFINITY;
@@ -388,24 +415,53 @@ __global__ __launch_bounds__(NW * 64, xa_waves(sizeof(T) == 4, KD)) void xa_rows
                         dlt[q] = d[q] + __shfl_xor(d[q], 32);
                     }
                 }
+                float top[QT];
+                auto gradients = [&]() __attribute__((always_inline)) {
 #pragma unroll
-                for (int kt = 0; kt < 4; ++kt) {
-                    if (!group_on(kt)) {
+                    for (int q = 0; q < QT; ++q) top[q] = 0.0f;
+#pragma unroll
+                    for (int kt = 0; kt < 4; ++kt) {
+                        if (!group_on(kt)) {
+#pragma unroll
+                            for (int q = 0; q < QT; ++q)
+#pragma unroll
+                                for (int r = 0; r < 4; ++r) pf[q].set(kt, r, 0.0f);
+                            continue;
+                        }
+                        floatx4 s[QT], dp[QT];
+                        scores(tk, kt, qf, s);
+                        scores(tv, kt, of, dp);
 #pragma unroll
                         for (int q = 0; q < QT; ++q)
 #pragma unroll
-                            for (int r = 0; r < 4; ++r) pf[q].set(kt, r, 0.0f);
-                        continue;
+                            for (int r = 0; r < 4; ++r) {
+                                float x;
+                                if constexpr (kScaled<T>) {
+                                    x = key_on(kt, r) ? prob(s, kt, q, r) * fmaf(dp[q][r], up[q], -dlt[q] * up[q]) : 0.0f;
+                                    top[q] = fmaxf(top[q], fabsf(x));
+                                } else x = key_on(kt, r) ? prob(s, kt, q, r) * (dp[q][r] - dlt[q]) : 0.0f;
+                                pf[q].set(kt, r, x);
+                            }
+                        __builtin_amdgcn_sched_barrier(0);
                     }
-                    floatx4 s[QT], dp[QT];
-                    scores(tk, kt, qf, s);
-                    scores(tv, kt, of, dp);
+                };
+                if constexpr (kScaled<T>) {
+#pragma unroll 1
+                    for (int turn = 0; turn < 2; ++turn) {          // a tile with a value that does not fit is formed again; infinities do not fit the second time either
+                        gradients();
+                        bool past = false;
 #pragma unroll
-                    for (int q = 0; q < QT; ++q)
+                        for (int q = 0; q < QT; ++q) past = past || top[q] > kUpLimit;
+                        if (!__any(past)) break;
 #pragma unroll
-                        for (int r = 0; r < 4; ++r) pf[q].set(kt, r, key_on(kt, r) ? prob(s, kt, q, r) * (dp[q][r] - dlt[q]) : 0.0f);
-                    __builtin_amdgcn_sched_barrier(0);
-                }
+                        for (int q = 0; q < QT; ++q) {
+                            const float by = fit(top[q]);
+                            up[q] *= by;
+#pragma unroll
+                            for (int d = 0; d < ND; ++d) acc[d][q] *= by;
+                        }
+                    }
+                } else gradients();
             }
             const unsigned tc = MODE == 2 ? tk : tv;
 #pragma unroll
@@ -478,6 +534,10 @@ __global__ __launch_bounds__(NW * 64, xa_waves(sizeof(T) == 4, KD)) void xa_rows
                 } else {
                     if (fg == 0) p.delta[flat] = dlt[t];
                     if (!p.dq.p) continue;
+                    if constexpr (kScaled<T>) {
+#pragma unroll
+                        for (int d = 0; d < ND; ++d) acc[d][t] *= 1.0f / up[t];
+                    }
                 }
                 const Strided& out = MODE == 0 ? p.o : p.dq;
                 T* o = (T*)(out.p + b * out.b + rs[t] * out.s + rh[t] * out.h);
@@ -533,8 +593,8 @@ __global__ __launch_bounds__(NW * 64, xa_waves(sizeof(T) == 4, KD)) void xa_keys
     extern __shared__ __attribute__((aligned(16))) char smem[];
     constexpr int TB = kTile * KD * 64, STAGE = 2 * TB + 2 * kTile * 4, STAGES = stages_of(KD, 2 * kTile * 4);      // Q and dO tiles, then lse and delta of the rows
     constexpr int KEYS = NW * KTW * 16;
-    // fp16 holds probabilities below 2^-14 with fewer bits, and with thousands of keys most are: dv is formed from 2^8 times them
-    constexpr float kUp = std::is_same_v<T, half_t> ? 256.0f : 1.0f;
+    // fp16 holds probabilities below 2^-14 with fewer bits, and with thousands of keys most are: dv is formed from 2^8 times them (8 less in the exponent's lse)
+    constexpr float kUpLog = kScaled<T> ? 8.0f : 0.0f, kDown = kScaled<T> ? 1.0f / 256.0f : 1.0f;
     const int tid = threadIdx.x, lane = tid & 63, wid = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int fr = lane & 15, fg = lane >> 4;
     int id = p.ragged ? blockIdx.x : xcd_chunk(blockIdx.x, gridDim.x);
@@ -553,8 +613,10 @@ __global__ __launch_bounds__(NW * 64, xa_waves(sizeof(T) == 4, KD)) void xa_keys
     bool key_ok[KTW];
     Frag<T> kf[KTW][KD], vf[KTW][KD];
     floatx4 ak[ND][KTW], av[ND][KTW];
+    float up[KTW];                                // kScaled: ps and ak hold up times their values
 #pragma unroll
     for (int j = 0; j < KTW; ++j) {
+        up[j] = kUpStart;
         key[j] = kbk * KEYS + (wid * KTW + j) * 16 + fr;
         key_ok[j] = key[j] < kv_len && (!p.mask || p.mask[b * p.mask_b + key[j]]);
         load_rows<T, KD>(kf[j], p.k.p + b * p.k.b + key[j] * p.k.s + hk * p.k.h, key_ok[j], p.D, lane);
@@ -595,7 +657,7 @@ __global__ __launch_bounds__(NW * 64, xa_waves(sizeof(T) == 4, KD)) void xa_keys
             row_delta = 0.0f;
             if (rr < rows) {
                 const long long at = ((long long)b * p.Sq + s) * p.H + hk * p.G + (rr - s * p.G);
-                row_lse = p.lse[at] * kLog2e;
+                row_lse = p.lse[at] * kLog2e - kUpLog;
                 if (row_lse == -INFINITY) row_lse = INFINITY;
                 row_delta = p.delta[at];
             }
@@ -621,6 +683,8 @@ __global__ __launch_bounds__(NW * 64, xa_waves(sizeof(T) == 4, KD)) void xa_keys
             const float* rl = (const float*)(smem + slot * STAGE + 2 * TB);
             if (active) {
             Probs<T> pp[KTW], ps[KTW];
+            floatx4 ds[kScaled<T> ? 4 : 1][KTW];
+            float top = 0.0f;
 #pragma unroll
             for (int rt = 0; rt < 4; ++rt) {
                 floatx4 s[KTW], dp[KTW];
@@ -638,9 +702,36 @@ __global__ __launch_bounds__(NW * 64, xa_waves(sizeof(T) == 4, KD)) void xa_keys
 #pragma unroll
                     for (int r = 0; r < 4; ++r) {
                         const float e = __builtin_amdgcn_exp2f(fmaf(s[j][r], p.scale2, -ls[r]));
-                        pp[j].set(rt, r, kUp == 1.0f ? e : e * kUp);          // a key that does not count has its own column of the results alone: set to zero at the end
-                        ps[j].set(rt, r, e * (dp[j][r] - dl[r]));
+                        pp[j].set(rt, r, e);          // a key that does not count has its own column of the results alone: set to zero at the end
+                        if constexpr (kScaled<T>) {
+                            ds[rt][j][r] = e * up[j] * (dp[j][r] - dl[r]);
+                            top = fmaxf(top, fabsf(ds[rt][j][r]));
+                        } else ps[j].set(rt, r, e * (dp[j][r] - dl[r]));
                     }
+            }
+            if constexpr (kScaled<T>) {
+                if (__any(top > kUpLimit)) {
+#pragma unroll
+                    for (int j = 0; j < KTW; ++j) {
+                        float m = 0.0f;
+#pragma unroll
+                        for (int rt = 0; rt < 4; ++rt)
+#pragma unroll
+                            for (int r = 0; r < 4; ++r) m = fmaxf(m, fabsf(ds[rt][j][r]));
+                        const float by = fit(m);
+                        up[j] *= by;
+#pragma unroll
+                        for (int rt = 0; rt < 4; ++rt) ds[rt][j] *= by;
+#pragma unroll
+                        for (int d = 0; d < ND; ++d) ak[d][j] *= by;
+                    }
+                }
+#pragma unroll
+                for (int j = 0; j < KTW; ++j)
+#pragma unroll
+                    for (int rt = 0; rt < 4; ++rt)
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) ps[j].set(rt, r, ds[rt][j][r]);
             }
 #pragma unroll
             for (int s2 = 0; s2 < Probs<T>::N; ++s2)
@@ -670,7 +761,8 @@ __global__ __launch_bounds__(NW * 64, xa_waves(sizeof(T) == 4, KD)) void xa_keys
         for (int d = 0; d < ND; ++d) {
             const int c = d * 16 + fg * 4;
             if (c >= p.D) continue;
-            const floatx4 none = {0.f, 0.f, 0.f, 0.f}, gk = key_ok[j] ? ak[d][j] * p.scale : none, gv = key_ok[j] ? av[d][j] * (1.0f / kUp) : none;
+            if constexpr (kScaled<T>) ak[d][j] *= kDown / up[j];
+            const floatx4 none = {0.f, 0.f, 0.f, 0.f}, gk = key_ok[j] ? ak[d][j] * p.scale : none, gv = key_ok[j] ? av[d][j] * kDown : none;
             if (part) { *(floatx4*)(part + c) = gk; *(floatx4*)(part + n + c) = gv; }
             else {
                 T4 wk, wv;
