@@ -15,11 +15,14 @@
 
 namespace {
 
-// ---- activations: act(g) and its slope.  exp and 1 / x are the hardware's (1 ulp).  The erf form uses Abramowitz & Stegun 7.1.26 for the tail
-// w = Phi(-|g|) = (a1 t + .. + a5 t^5) exp(-g^2 / 2) / 2, t = 1 / (1 + p |g| / sqrt 2), off by at most 7.5e-8; act = max(g, 0) - |g| w has no
-// difference of near values.  12 plain and 2 transcendental instructions; the library's erff took about 40 and made the epilogue of short-K products the bound.
+// ---- activations: act(g) and its slope.  exp and 1 / x are the hardware's (1 ulp).  The erf form takes the tail w = Phi(-|g|) = t Q(t) exp(-g^2 / 2), t = 1 / (1 + p |g|);
+// act = max(g, 0) - |g| w has no difference of near values.
+// 16-bit types: Abramowitz & Stegun 7.1.26, Q of five terms, w off by at most 7.5e-8 absolutely (relatively 5e-5 at |g| = 3, 1.6e-3 at 5, 1e-2 at 8).  12 plain and 2 transcendental
+// instructions; the library's erff took about 40 and made the epilogue of short-K products the bound.
+// fp32, whose products leave the epilogue time: Q of nine terms, fitted to erfcx(|g| / sqrt 2) / (2 t) for the least relative error on 0 <= |g| <= 13.3 (1.0e-8; past that w is less
+// than fp32's smallest normal value), so that gates far out on the negative side keep their precision: act is off by (g^2 + 32) 2^-24 of itself, the g^2 from the exponential's argument.
 __device__ __forceinline__ float exp_of(float x) { return __builtin_amdgcn_exp2f(x * 1.4426950408889634f); }
-template <int ACT> __device__ __forceinline__ void activation(float g, float& act, float& slope)
+template <typename T, int ACT> __device__ __forceinline__ void activation(float g, float& act, float& slope)
 {
     if constexpr (ACT == SDE_ACT_SILU) {
         const float s = __builtin_amdgcn_rcpf(1.0f + exp_of(-g));
@@ -27,12 +30,25 @@ template <int ACT> __device__ __forceinline__ void activation(float g, float& ac
         slope = s * (1.0f + g * (1.0f - s));
     } else if constexpr (ACT == SDE_ACT_GELU) {
         const float ax = fabsf(g);
-        const float t = __builtin_amdgcn_rcpf(fmaf(0.23164189f, ax, 1.0f));            // p / sqrt 2, p = 0.3275911
-        const float e = __builtin_amdgcn_exp2f(g * g * -0.72134752f);                  // exp(-g^2 / 2)
-        float w = fmaf(0.5307027145f, t, -0.7265760135f);                              // a5 / 2 .. a1 / 2
-        w = fmaf(w, t, 0.7107068705f);
-        w = fmaf(w, t, -0.142248368f);
-        w = fmaf(w, t, 0.127414796f);
+        const float e = __builtin_amdgcn_exp2f(g * g * -0.72134752f);                      // exp(-g^2 / 2)
+        float t, w;
+        if constexpr (sizeof(T) == 4) {
+            t = __builtin_amdgcn_rcpf(fmaf(0.26452443f, ax, 1.0f));
+            w = fmaf(0.0310996249f, t, -0.146480367f);
+            w = fmaf(w, t, 0.223770157f);
+            w = fmaf(w, t, -0.122620679f);
+            w = fmaf(w, t, 0.142120138f);
+            w = fmaf(w, t, 0.0586104058f);
+            w = fmaf(w, t, 0.102940425f);
+            w = fmaf(w, t, 0.105005592f);
+            w = fmaf(w, t, 0.105554707f);
+        } else {
+            t = __builtin_amdgcn_rcpf(fmaf(0.23164189f, ax, 1.0f));                        // p / sqrt 2, p = 0.3275911
+            w = fmaf(0.5307027145f, t, -0.7265760135f);                                    // a5 / 2 .. a1 / 2
+            w = fmaf(w, t, 0.7107068705f);
+            w = fmaf(w, t, -0.142248368f);
+            w = fmaf(w, t, 0.127414796f);
+        }
         w = w * t * e;
         act = fmaf(-fminf(ax, 64.0f), w, fmaxf(g, 0.0f));                              // an infinite gate: infinity times 0 is not wanted here
         slope = fmaf(g * 0.3989422804014327f, e, g >= 0.0f ? 1.0f - w : w);
@@ -319,7 +335,7 @@ __global__ __launch_bounds__(TileOf<CFG>::type::threads) void gff_gemm_kernel(Gf
                         const int i = q * 4 + r;
                         const float a = acc[q][mt][r] + bv[i], g = acc[q + P][mt][r] + bg[i];
                         float act, slope;
-                        activation<ACT>(g, act, slope);
+                        activation<T, ACT>(g, act, slope);
                         if constexpr (EPI == GFF_FWD) o1[mt][q][r] = (T)(a * act);
                         else {
                             // rounded to the inputs' type once: they are operands of the next two products; the bias gradient takes them unrounded
