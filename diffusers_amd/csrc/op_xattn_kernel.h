@@ -797,24 +797,6 @@ template <typename T> __global__ __launch_bounds__(256) void xa_keys_join_kernel
     }
 }
 
-// rows without keys (or no keys at all): zeros, lse -inf
-template <typename T> __global__ __launch_bounds__(256) void xa_zero_kernel(Strided x, int S, int H, int D, long long n, float* lse)
-{
-    for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < n; i += (long long)gridDim.x * 256) {
-        const long long bs = i / D / H;
-        const int h = (int)(i / D % H), d = (int)(i % D);
-        if (x.p) ((T*)(x.p + bs / S * x.b + bs % S * x.s + h * x.h))[d] = (T)0.0f;
-        if (lse && d == 0) lse[bs * H + h] = -INFINITY;
-    }
-}
-template <typename T> void xa_zero(const OpCtx& c, const Strided& x, int B, int S, int H, int D, float* lse)
-{
-    const long long n = (long long)B * S * H * D;
-    if (n == 0 || (!x.p && !lse)) return;
-    xa_zero_kernel<T><<<(unsigned)std::min<long long>(cdiv64(n, 256), 4096), 256, 0, c.stream>>>(x, S, H, D, n, lse);
-    op_launched("cross attention zeros");
-}
-
 template <typename T, int KD, int ND, int NW, int QT, int MODE, bool RES> void xa_rows(const OpCtx& c, const XaDev& d)
 {
     constexpr int smem = stages_of(KD, 0) * 2 * kTile * KD * 64;

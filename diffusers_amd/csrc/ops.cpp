@@ -82,19 +82,18 @@ void check(const sde_cross_attention_args* a)
     const int64_t groups = a->B * a->Hkv * std::max((a->Sq * (a->H / a->Hkv) + 15) / 16, (a->Skv + 63) / 64);
     need(groups < kMaxRows, "cross attention: too many workgroups");
 }
-void tensor(const sde_cross_attention_args& a, const void* p, const int64_t* s, int64_t S, int64_t H, const char* what)
+void tensor(const sde_cross_attention_args& a, const void* p, const int64_t* s, int64_t H, const char* what)
 {
     const int64_t e = (int64_t)op_esize(a.dtype);
     bool ok = p && ((uintptr_t)p & 15) == 0;
     for (int i = 0; i < 3; ++i) ok = ok && s[i] >= 0 && s[i] < (int64_t(1) << 40) && s[i] * e % 16 == 0;
     ok = ok && (65 * s[1] + H * s[2] + a.D) * e < kMaxRows;
     if (!ok) sde_fail(SDE_ERR_INVALID_ARGUMENT, std::string("cross attention: ") + what + " is null, not 16-byte aligned, or a stride does not fit");
-    (void)S;
 }
 // an output's elements must not share memory
 void output(const sde_cross_attention_args& a, const void* p, const int64_t* s, int64_t S, int64_t H, const char* what)
 {
-    tensor(a, p, s, S, H, what);
+    tensor(a, p, s, H, what);
     int64_t size[3] = {a.B, S, H}, str[3] = {s[0], s[1], s[2]};
     for (int i = 0; i < 3; ++i)                       // by stride, smallest first
         for (int j = i + 1; j < 3; ++j)
@@ -213,9 +212,9 @@ sde_status sde_cross_attention_forward(const sde_cross_attention_args* a, const 
         if (a->B && a->Sq) {
             output(*a, a->o, a->o_stride, a->Sq, a->H, "o");
             if (a->Skv) {
-                tensor(*a, a->q, a->q_stride, a->Sq, a->H, "q");
-                tensor(*a, a->k, a->k_stride, a->Skv, a->Hkv, "k");
-                tensor(*a, a->v, a->v_stride, a->Skv, a->Hkv, "v");
+                tensor(*a, a->q, a->q_stride, a->H, "q");
+                tensor(*a, a->k, a->k_stride, a->Hkv, "k");
+                tensor(*a, a->v, a->v_stride, a->Hkv, "v");
             }
         }
         run(exec, op_cross_attention_ws_bytes(*a, false), [&](const OpCtx& c) { op_cross_attention_forward(c, *a); });
@@ -231,11 +230,11 @@ sde_status sde_cross_attention_backward(const sde_cross_attention_args* a, const
         if (a->dk && a->B && a->Skv) output(*a, a->dk, a->dk_stride, a->Skv, a->Hkv, "dk");
         if (a->dv && a->B && a->Skv) output(*a, a->dv, a->dv_stride, a->Skv, a->Hkv, "dv");
         if (a->B && a->Sq && a->Skv) {
-            tensor(*a, a->q, a->q_stride, a->Sq, a->H, "q");
-            tensor(*a, a->k, a->k_stride, a->Skv, a->Hkv, "k");
-            tensor(*a, a->v, a->v_stride, a->Skv, a->Hkv, "v");
-            tensor(*a, a->o, a->o_stride, a->Sq, a->H, "o");
-            tensor(*a, a->d_o, a->do_stride, a->Sq, a->H, "d_o");
+            tensor(*a, a->q, a->q_stride, a->H, "q");
+            tensor(*a, a->k, a->k_stride, a->Hkv, "k");
+            tensor(*a, a->v, a->v_stride, a->Hkv, "v");
+            tensor(*a, a->o, a->o_stride, a->H, "o");
+            tensor(*a, a->d_o, a->do_stride, a->H, "d_o");
             need(a->lse != nullptr, "cross attention: lse is null");
         }
         run(exec, op_cross_attention_ws_bytes(*a, true), [&](const OpCtx& c) { op_cross_attention_backward(c, *a); });
