@@ -30,6 +30,14 @@ constexpr int xa_ktw(bool f32, int kd) { return f32 ? (kd >= 4 ? 1 : 2) : (kd >=
 constexpr int xa_waves(bool f32, int kd) { return kd >= (f32 ? 8 : 6) ? 1 : 2; }
 // 16-row groups of a wave: two where q, o and the scores of 32 rows (dq: do too) fit into 256 registers.  Head size 128, us, one / two groups: forward 140 / 120, dq 159 / 217.
 constexpr int xa_qt(int kd, bool dq) { return kd >= (dq ? 4 : 5) ? 1 : 2; }
+// Stages of a kernel whose stage holds two tiles (and `extra` bytes).  Two, unless they leave one workgroup to a CU where one stage leaves three (head size 160, fp16, dk / dv with dq 104 us with two
+// stages, 87 with one), or do not fit at all (fp32 heads past 128).
+constexpr int xa_stage(int kd, int extra) { return 2 * kTile * kd * 64 + extra; }
+constexpr int stages_of(int kd, int extra)
+{
+    const int s = xa_stage(kd, extra), lds = 160 * 1024;
+    return 4 * s <= lds ? 2 : 3 * s <= lds ? 1 : 2 * s <= lds - 1024 ? 2 : 1;
+}
 void xa_forward_f16(const OpCtx& c, const XaPlan& p, const XaDev& d);
 void xa_forward_bf16(const OpCtx& c, const XaPlan& p, const XaDev& d);
 void xa_forward_f32(const OpCtx& c, const XaPlan& p, const XaDev& d);

@@ -68,8 +68,8 @@ XaPlan xa_plan(const sde_cross_attention_args& a)
     const int64_t blocks = heads * p.fwd.nrb, want = p.fwd.nw == 1 ? 2048 : 512;
     p.splits = 1;
     if (blocks < 256 || (p.fwd.nw == 1 && blocks < want)) p.splits = (int)std::max<int64_t>(1, std::min<int64_t>({want / blocks, ktiles / 2, 64}));
-    // two tiles of keys or fewer stay in LDS while a workgroup walks blocks of rows over them: as many as leave 4 workgroups to a CU
-    if (R > 64 && ktiles <= 2) {
+    // two tiles of keys or fewer stay in LDS, where it has two stages, while a workgroup walks blocks of rows over them: as many as leave 4 workgroups to a CU
+    if (R > 64 && ktiles <= 2 && stages_of(p.kd, 0) == 2) {
         auto blocks_of = [&](const XaRows& r) { return (int)std::max<int64_t>(1, std::min<int64_t>(heads * r.nrb / 1024, 16)); };
         p.fwd.rpg = p.splits == 1 ? blocks_of(p.fwd) : 0;
         p.dq.rpg = blocks_of(p.dq);
@@ -103,6 +103,14 @@ XaDev xa_dev(const sde_cross_attention_args& a)
 }
 
 }  // namespace
+
+int64_t op_cross_attention_threads(const sde_cross_attention_args& a)
+{
+    if (!a.B || !a.Sq || !a.Skv) return 0;
+    const XaPlan p = xa_plan(a);
+    auto rows = [&](const XaRows& r, int64_t splits) { return (r.rpg ? cdiv64(r.nrb, r.rpg) : r.nrb) * splits * r.nw * 64; };
+    return a.B * a.Hkv * std::max({rows(p.fwd, p.splits), rows(p.dq, 1), (int64_t)p.nkb * p.key_splits * 256});
+}
 
 size_t op_cross_attention_ws_bytes(const sde_cross_attention_args& a, bool backward)
 {

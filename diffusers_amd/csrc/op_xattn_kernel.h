@@ -8,15 +8,6 @@
 
 namespace {
 
-// Stages of a kernel whose stage holds two tiles (and `extra` bytes).  Two, unless they leave one workgroup to a CU where one stage leaves three (head size 160, fp16, dk / dv with dq 104 us with two
-// stages, 87 with one), or do not fit at all (fp32 heads past 128).
-constexpr int xa_stage(int kd, int extra) { return 2 * kTile * kd * 64 + extra; }
-constexpr int stages_of(int kd, int extra)
-{
-    const int s = xa_stage(kd, extra), lds = 160 * 1024;
-    return 4 * s <= lds ? 2 : 3 * s <= lds ? 1 : 2 * s <= lds - 1024 ? 2 : 1;
-}
-
 template <typename T> struct Cfg { static constexpr int frag = 64 / (int)sizeof(T); };   // elements of a 64-byte step of a contraction
 
 __device__ __forceinline__ int xcd_chunk(int bid, int n)
@@ -812,7 +803,7 @@ template <typename T, int KD, int ND, int MODE> void xa_rows_by(const OpCtx& c, 
     d.nrb = r.nrb;
     d.rpg = r.rpg;
     if (r.nw == 1) { xa_rows<T, KD, ND, 1, 1, MODE, false>(c, d); return; }
-    if constexpr (MODE != 1 && stages_of(KD, 0) == 2) {              // the keys' two tiles need two stages
+    if constexpr (MODE != 1 && stages_of(KD, 0) == 2) {              // as xa_plan has it
         if (d.rpg) { xa_rows<T, KD, ND, 4, QT, MODE, true>(c, d); return; }
     }
     if constexpr (QT == 2) {

@@ -58,6 +58,7 @@ void check(const sde_gated_ff_args* a)
     need(a->K > 0 && a->K <= (1 << 22) && a->K % v == 0, "gated ff: K must be a positive multiple of 16 bytes");
     need(a->F > 0 && a->F <= (1 << 22) && a->F % v == 0, "gated ff: F must be a positive multiple of 16 bytes");
     need((a->M + 255) / 256 * ((a->F + 127) / 128) < kMaxRows, "gated ff: M times F is too large");
+    need(a->M < kMaxRows - 256, "gated ff: M is too large");          // a whole K-tile past M is still counted in 32 bits
 }
 // a matrix of the gated feed-forward: aligned, rows that do not overlap, 256 of them inside a 31-bit window
 void matrix(const sde_gated_ff_args& a, const void* p, int64_t ld, int64_t cols, const char* what)
@@ -78,9 +79,7 @@ void check(const sde_cross_attention_args* a)
     need(a->Sq * (a->H / a->Hkv) < kMaxRows - 4096, "cross attention: too many query rows");
     need(a->B * a->Hkv < (1 << 24), "cross attention: B times Hkv is too large");
     need(!a->key_mask || a->B <= 1 || a->key_mask_stride >= a->Skv, "cross attention: key_mask_stride is less than Skv");
-    // one workgroup to 16 rows (64 keys) at the least, each in at most 64 parts
-    const int64_t groups = a->B * a->Hkv * std::max((a->Sq * (a->H / a->Hkv) + 15) / 16, (a->Skv + 63) / 64);
-    need(groups < kMaxRows, "cross attention: too many workgroups");
+    need(op_cross_attention_threads(*a) < (int64_t(1) << 32), "cross attention: too many workgroups");
 }
 void tensor(const sde_cross_attention_args& a, const void* p, const int64_t* s, int64_t H, const char* what)
 {

@@ -19,6 +19,7 @@ struct GffPlan { int cfg, splits; };                                            
 GffPlan op_gated_ff_plan(const sde_gated_ff_args& a, int product, int64_t* units);  // product: 0 = x W^T, 1 = dx, 2 = dW; units: tiles times parts
 
 size_t op_cross_attention_ws_bytes(const sde_cross_attention_args& a, bool backward);
+int64_t op_cross_attention_threads(const sde_cross_attention_args& a);             // of the largest launch: HIP takes less than 2^32
 void op_cross_attention_forward(const OpCtx& c, const sde_cross_attention_args& a);
 void op_cross_attention_backward(const OpCtx& c, const sde_cross_attention_args& a);
 

@@ -41,3 +41,30 @@ def test_plans_of_known_sizes_are_as_they_were():
 @pytest.mark.parametrize("product", [-1, 3])
 def test_the_plan_refuses_an_unknown_product(product):
     assert L.sde_test_gated_ff_plan(ff(0, 4, 64, 64), product, C.c_int(), C.c_int(), C.c_int64()) == 1
+
+
+def xa(**kw):
+    a = dict(dtype=1, B=2, Sq=3, Skv=7, H=4, Hkv=2, D=64, scale=0.125, q=P, k=P, v=P, o=P, lse=P, d_o=P, dq=P, dk=P, dv=P)
+    return _lib.CrossAttentionArgs(**{**a, **kw})
+
+
+@pytest.mark.parametrize("sizes,fits", [({"B": 1 << 20, "Hkv": 15, "H": 15, "D": 8, "Sq": 1, "Skv": 64}, True), ({"B": 1 << 20, "Hkv": 15, "H": 15, "D": 8, "Sq": 1, "Skv": 128}, True),
+                                        ({"B": 1 << 20, "Hkv": 15, "H": 15, "D": 8, "Sq": 1, "Skv": 129}, False), ({"B": 1 << 20, "Hkv": 15, "H": 15, "D": 8, "Sq": 17, "Skv": 64}, True),
+                                        ({"B": 1 << 20, "Hkv": 15, "H": 15, "D": 8, "Sq": 65, "Skv": 64}, True), ({"B": 1 << 20, "Hkv": 15, "H": 15, "D": 8, "Sq": 2049, "Skv": 200}, False),
+                                        ({"B": 1 << 22, "Hkv": 1, "H": 1, "D": 256, "Sq": 1, "Skv": 320}, False), ({"B": 1 << 20, "Hkv": 15, "H": 15, "D": 8, "Sq": 0, "Skv": 10000}, True)])
+def test_launches_that_the_hardware_does_not_take_are_refused_before_anything_runs(sizes, fits):
+    """A launch has less than 2^32 threads: 256 of them to 64 or 128 keys of a key head, 64 or 256 to a block of rows."""
+    n = C.c_size_t()
+    status = L.sde_cross_attention_workspace(xa(**sizes), 1, n)
+    assert status == (0 if fits else 1)
+    if not fits:
+        assert b"too many workgroups" in L.sde_last_error()
+
+
+@pytest.mark.parametrize("m,fits", [((1 << 31) - 257, True), ((1 << 31) - 256, False), ((1 << 31) - 1, False)])
+def test_rows_of_gated_ff_past_what_a_contraction_counts(m, fits):
+    """dW runs over the rows in steps of 64 counted in 32 bits: the last 64 rows before 2^31 came out as no rows at all."""
+    status = L.sde_gated_ff_workspace(ff(1, m, 8, 8), 1, C.c_size_t())
+    assert status == (0 if fits else 1)
+    if not fits:
+        assert b"too large" in L.sde_last_error()
