@@ -109,3 +109,33 @@ def test_what_the_library_refuses_in_a_backward_pass_is_its_own_error():
     with pytest.raises(_lib.SdeError, match="too large") as e:
         torch.autograd.grad(h, w, torch.ones_like(h))
     assert e.value.status == 1
+
+
+@pytest.mark.parametrize("name", ["layer_norm", "gated_ff", "cross_attention"])
+def test_several_upstream_gradients_at_once(name):
+    """is_grads_batched: the backward pass for each of them."""
+    f, args = case(name)
+    leaves = leaves_of(args)
+    y = f(*args)
+    dy = r(3, *y.shape, seed=31)
+    got = torch.autograd.grad(y, leaves, dy, is_grads_batched=True, retain_graph=True)
+    for i in range(3):
+        assert all(torch.equal(a[i], b) for a, b in zip(got, torch.autograd.grad(y, leaves, dy[i], retain_graph=True)))
+
+
+@pytest.mark.parametrize("name", ["layer_norm", "gated_ff", "cross_attention"])
+def test_functional_transforms_are_right_or_refused(name):
+    f, args = case(name)
+    g = lambda x: f(x, *args[1:])
+    assert torch.equal(torch.func.vmap(g)(torch.stack([args[0], 2 * args[0]])), torch.stack([g(args[0]), g(2 * args[0])]))
+    assert torch.equal(torch.func.functionalize(g)(args[0]), g(args[0]))
+    for transform in (torch.func.grad(lambda x: g(x).float().sum()), torch.func.jacrev(g), lambda x: torch.func.jvp(g, (x,), (x,))):
+        with pytest.raises(RuntimeError):
+            transform(args[0])
+
+
+@pytest.mark.parametrize("name", ["layer_norm", "gated_ff", "cross_attention"])
+def test_torchs_own_checks_of_an_operator(name):
+    args = {"layer_norm": case(name)[1], "gated_ff": [*case(name)[1], 2], "cross_attention": case(name)[1][:3]}[name]
+    leaves_of([t for t in args if isinstance(t, torch.Tensor)])
+    torch.library.opcheck(getattr(torch.ops.diffusers_amd, name).default, tuple(args), test_utils=("test_schema", "test_autograd_registration", "test_faketensor"))
