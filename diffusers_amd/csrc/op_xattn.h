@@ -24,11 +24,15 @@ struct XaDev {
 // keys (0: they do not fit)
 struct XaRows { int nw, qt, nrb, rpg; };
 struct XaPlan { int kd, nd; XaRows fwd, dq; int splits, nkb, key_splits, chunk; };
-// 16-key groups of a wave that owns keys: two where K, V and both gradients of 32 keys fit into its registers
+// 16-key groups of a wave that owns keys: two while K, V and both gradients of 32 keys leave its registers room, one past that.  dk, dv, us, one / two groups, 4 sequences of 8 heads: fp16, 4096
+// rows and keys, head size 32 253 / 224, 64 360 / 315; 2048 of 96 154 / 123, but with few keys, which leave few workgroups of twice the keys, 34 / 47 (1000 rows on 333); bf16 of 128
+// spills.  fp32, 2048 of 32 285 / 284, of 64 555 / 525, but 48 / 59 (333 rows on 1000).
 constexpr int xa_ktw(bool f32, int kd) { return f32 ? (kd >= 4 ? 1 : 2) : (kd >= 3 ? 1 : 2); }
 // waves of a SIMD the registers are shared out for
 constexpr int xa_waves(bool f32, int kd) { return kd >= (f32 ? 8 : 6) ? 1 : 2; }
-// 16-row groups of a wave: two where q, o and the scores of 32 rows (dq: do too) fit into 256 registers.  Head size 128, us, one / two groups: forward 140 / 120, dq 159 / 217.
+// 16-row groups of a wave: two where q, o and the scores of 32 rows (dq: do too) fit into 256 registers of every type's kernel.  us, one / two groups, 4 sequences of 8 heads, 2048 rows and keys:
+// forward fp16 64 (4096) 220 / 200, 96 93 / 72, bf16 128 116 / 88, fp16 160 133 / 222 (spills), fp32 64 295 / 284, 80 373 / 343 and equal with fewer rows; dq fp16 96 130 / 97, bf16 128 132 / 110,
+// but fp16 128 142 / 167 (8 ragged sequences; spills), fp32 64 424 / 402, but 66 / 111 with 333 rows (half the workgroups).
 constexpr int xa_qt(int kd, bool dq) { return kd >= (dq ? 4 : 5) ? 1 : 2; }
 // Stages of a kernel whose stage holds two tiles (and `extra` bytes).  Two, unless they leave one workgroup to a CU where one stage leaves three (head size 160, fp16, dk / dv with dq 104 us with two
 // stages, 87 with one), or do not fit at all (fp32 heads past 128).

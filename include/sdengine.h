@@ -300,8 +300,10 @@ sde_status sde_rng_seed_key(uint64_t seed, uint8_t key_out[32]);
  *     call may be captured into a graph.  The caller's current device is left as it was;
  *   - `workspace` (256-byte aligned) is scratch for this call: at least what the matching *_workspace says for the same arguments.  It may
  *     be used again by later work on the same stream, not by work that may run at the same time;
- *   - dtype: sde_dtype of the tensors.  All sums, statistics and softmax terms are fp32; results are rounded once at the end, operands of a
- *     product in the backward passes once more.  No atomics: the same call gives the same bits;
+ *   - dtype: sde_dtype of the tensors.  All sums and statistics are fp32 and results are rounded once at the end.  Operands that a product inside takes are rounded to the
+ *     tensors' type too: the probabilities (for dv, and for o where a key head has more than 16 rows), the score gradients (for dq and dk), the gradients of the gated
+ *     feed-forward's two projections (for dx and dweight), and, with more than 64 keys, the o that delta is formed from.  fp16: score gradients, and probabilities for dv, are scaled by powers
+ *     of two on the way, so that small ones keep their bits.  No atomics: the same call gives the same bits;
  *   - sizes may be zero; strides and leading dimensions are in ELEMENTS, the last axis has stride 1.  Arguments that are not met are refused with
  *     SDE_ERR_INVALID_ARGUMENT before anything is enqueued.  Outputs may not overlap inputs unless stated. */
 typedef struct sde_op_exec {
@@ -337,7 +339,7 @@ sde_status sde_layer_norm_workspace(const sde_layer_norm_args* a, size_t* bytes)
 
 /* h = (x Wv^T + bv) * act(x Wg^T + bg): x [M, K]; weight [2F, K] with the F value rows first, then the F gate rows (the order of the file's
  * GEGLU projection); bias [2F] of bias_dtype (= dtype or SDE_F32) or NULL; h [M, F].  K and F are multiples of 8 (SDE_F32: 4), all tensors start on
- * 16 bytes and their leading dimensions are multiples of 16 bytes and less than 8 MB.
+ * 16 bytes and their leading dimensions are multiples of 16 bytes and less than 8 MB.  M < 2^31 - 256; backward: F < 2^21.
  * SDE_ACT_GELU: the tail Phi(-|g|) is good to a few units of fp32's last place for SDE_F32 and to 7.5e-8, absolutely, for the 16-bit types.
  * Backward: dh [M, F] -> dx [M, K], dweight [2F, K], dbias [2F] of bias_dtype, each may be NULL.  The pre-activations are formed again from x and
  * weight; the workspace holds the two gradients of the projections ([M, 2F]). */
