@@ -386,7 +386,8 @@ __global__ __launch_bounds__(NW * 64, xa_waves(sizeof(T) == 4, KD)) void xa_rows
                 auto prob = [&](const floatx4 (&x)[QT], int kt, int q, int r) { return key_on(kt, r) ? __builtin_amdgcn_exp2f(fmaf(x[q][r], p.scale2, -lse2[q])) : 0.0f; };
                 if (ntiles == 1) {
                     // All keys are here: delta = sum of p dp, without the rounding of o.  With few keys that rounding, u |do| |o|, is as large as those of the products'
-                    // operands; with many keys o is a mean and it is small.
+                    // operands; with many keys o is a mean and it is small, unless one key takes most of a row (bf16, 300 keys: dq is 2.4e-3 off for N(0, 1) scores, 4.6e-3 where the
+                    // largest probability is 0.65 on average, 5.9e-3 at 0.83; fp16 3.0e-4, 5.8e-4, 7.7e-4).  A second walk over the keys would take it away, for half as much time again.
                     float d[QT];
 #pragma unroll
                     for (int q = 0; q < QT; ++q) d[q] = 0.0f;
