@@ -136,10 +136,10 @@ template <typename T> struct Probs {
 // Score gradients ds = p (dp - delta) as fp16 operands.  p is about 1 / Skv and the upstream gradient any size, so ds itself lies where fp16 has few bits or none (2^-24 and less: with 8000 keys
 // and do of 1e-3 the products with it were 1 % off) or past its largest value.  They go in as 2^n ds, each column of the product (a row for dq, a key for dk) with an n of its own: it starts
 // high and comes down, with the sums so far, when a value passes 2^15, to put that value at 2^8 .. 2^9.  Powers of two: exact.  bf16 and fp32 have the range.
-// dk / dv: starts at 2^80, the first tile brings it down.  Backward pass of fp16, us before / with: 8 x 2047 x 16 heads of 128 (4 shared) on 1500 keys 908 / 890, 16 x 4096 x 8 of 40 on 77
+// dk / dv: starts at 2^72, the first tile brings it down.  Backward pass of fp16, us before / with: 8 x 2047 x 16 heads of 128 (4 shared) on 1500 keys 908 / 890, 16 x 4096 x 8 of 40 on 77
 // 96 / 100, 2 x 4096 x 8 of 40 on 4096 257 / 259.
 template <typename T> constexpr bool kScaled = std::is_same_v<T, half_t>;
-constexpr float kUpStart = 1.2089258196146292e24f, kUpLimit = 32768.0f;      // 2^80: times the largest |dp - delta| (256 products of 65504^2) it is still finite
+constexpr float kUpStart = 4.722366482869645e21f, kUpLimit = 32768.0f;       // 2^72: times 2^8 p (dk / dv) and the largest |dp - delta|, twice 256 products of 65504^2, it is still finite
 __device__ __forceinline__ unsigned exponent(float m) { return __builtin_bit_cast(unsigned, m) >> 23; }          // of m >= 0: 127 and up from 1, 255 for infinity
 __device__ __forceinline__ float to_2_8(unsigned e) { return __builtin_bit_cast(float, (127 + 8 + 127 - e) << 23); }      // brings a value of this exponent to 2^8 .. 2^9
 // what a column is multiplied with so that its largest magnitude (this lane's is `m`; a column is lanes l, l + 16, + 32, + 48) fits

@@ -133,3 +133,19 @@ def test_shared_heads_and_lengths():
                 near(dq[b, :ql[b], 3 * h + i], wq, f"dq {b} {h} {i}")
                 sum_k = sum_k + wk
             near(dk[b, :kl[b], h], sum_k, f"dk {b} {h}")
+
+
+@pytest.mark.parametrize("d", [64, 256])
+@pytest.mark.parametrize("keys", [2, 100])
+def test_the_largest_gradients_that_can_be(keys, d):
+    """do and v at fp16's largest values, their signs alike in half of the keys: dp is up to D 65504^2.  The scale brings the results back into range."""
+    g = torch.Generator(device="cuda").manual_seed(keys + d)
+    q, k = (torch.randn(n, d, generator=g, device="cuda").half() for n in (70, keys))
+    sign = torch.where(torch.rand(d, generator=g, device="cuda") < 0.5, -1.0, 1.0)
+    v = (65504 * sign * torch.where(torch.arange(keys, device="cuda") % 2 == 0, 1.0, -1.0)[:, None]).half()
+    do = (65504 * sign).expand(70, d).half()
+    scale = 2.0 ** -28
+    want = gradients(q, k, v, do, scale)
+    assert all(1 < w.abs().max() < 60000 for w in want[:2])
+    for name, a, b in zip(("dq", "dk"), run(q, k, v, do, scale), want):
+        near(a, b, name)
