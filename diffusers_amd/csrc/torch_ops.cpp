@@ -95,7 +95,7 @@ bool wants(const Tensor& t) { return t.defined() && t.requires_grad(); }
 bool wants(const MaybeTensor& t) { return t && wants(*t); }
 
 // Tensors without memory (shapes alone, a tracer's) count as aligned: the launch looks again.
-bool has_memory(const Tensor& x) { return !x.is_meta() && !at::isTensorSubclassLike(x); }
+bool has_memory(const Tensor& x) { return !x.is_meta() && (x.key_set() & at::kTensorSubclassLike).empty(); }
 bool aligned(const Tensor& x, int64_t align) { return align == 1 || !has_memory(x) || (uintptr_t)x.data_ptr() % align == 0; }
 
 // x [..., cols] as rows: elements from row to row, -1 where the leading axes have no one step

@@ -73,3 +73,23 @@ def test_a_step_from_outside_of_the_capture():
         g.replay()
         torch.cuda.synchronize()
         assert torch.equal(gw, want)
+
+
+def test_refused_under_a_dispatch_mode_too():
+    from torch.utils._python_dispatch import TorchDispatchMode
+
+    class Watch(TorchDispatchMode):
+        def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+            return func(*args, **(kwargs or {}))
+
+    x, w = r(4, 64, seed=1), r(64, seed=2).requires_grad_()
+    alive = ops.layer_norm(x, w)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        with Watch(), pytest.raises(RuntimeError, match="alive"):
+            ops.layer_norm(x, w)
+        with torch.no_grad():
+            y = ops.layer_norm(x, w)
+    g.replay()
+    assert torch.equal(y, alive)
