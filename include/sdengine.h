@@ -342,7 +342,7 @@ sde_status sde_layer_norm_workspace(const sde_layer_norm_args* a, size_t* bytes)
  * 16 bytes and their leading dimensions are multiples of 16 bytes and less than 8 MB.  M < 2^31 - 256; backward: F < 2^21.
  * SDE_ACT_GELU: the tail Phi(-|g|) is good to a few units of fp32's last place for SDE_F32 and to 7.5e-8, absolutely, for the 16-bit types.
  * Backward: dh [M, F] -> dx [M, K], dweight [2F, K], dbias [2F] of bias_dtype, each may be NULL.  The pre-activations are formed again from x and
- * weight; the workspace holds the two gradients of the projections ([M, 2F]). */
+ * weight; the workspace holds the two gradients of the projections ([M, 2F]) in the tensors' type (SDE_F16: like any gradient in it, below 2^-14 with fewer bits; scale dh if it is that small). */
 typedef enum sde_activation { SDE_ACT_GELU = 0, SDE_ACT_GELU_TANH = 1, SDE_ACT_SILU = 2 } sde_activation;
 typedef struct sde_gated_ff_args {
     int dtype, bias_dtype, activation;
